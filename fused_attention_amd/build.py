@@ -6,16 +6,19 @@ standalone `test` executable).  Here the device code is compiled once by hipcc f
 a plain shared library with a C ABI, and the torch binding is host-only C++ compiled by g++
 that links against it, so no source ever passes through a CUDA-to-HIP translation step.
 """
+import concurrent.futures
 import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libfused_attn_gfx950.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
+LIB_SOURCES = ["fused_attn_capi.hip", "fused_attn_cache.hip"]
 SMOKE_PATH = os.path.join(PKG_DIR, "fa_test")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
@@ -51,8 +54,12 @@ def _run(cmd):
 
 def build_kernel_library():
     hipcc = os.path.join(ROCM, "bin", "hipcc")
-    _run([hipcc] + HIPCC_FLAGS + ["-fPIC", "-shared",
-                                  os.path.join(CSRC, "fused_attn_capi.hip"), "-o", LIB_PATH])
+    # one translation unit each, compiled at the same time
+    with tempfile.TemporaryDirectory() as where, concurrent.futures.ThreadPoolExecutor() as pool:
+        objects = [os.path.join(where, name + ".o") for name in LIB_SOURCES]
+        list(pool.map(lambda name, obj: _run([hipcc] + HIPCC_FLAGS + ["-fPIC", "-c", os.path.join(CSRC, name), "-o", obj]),
+                      LIB_SOURCES, objects))
+        _run([hipcc, "--offload-arch=gfx950", "-shared"] + objects + ["-o", LIB_PATH])
     return LIB_PATH
 
 

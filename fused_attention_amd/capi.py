@@ -13,11 +13,19 @@ LIB_PATH = os.path.join(_PKG_DIR, "libfused_attn_gfx950.so")
 
 # every symbol include/fused_attn.h declares
 EXPORTS = ("fa_fwd", "fa_fwd_ex", "fa_fwd_strided", "fa_fwd_plan", "fa_fwd_variant", "fa_fwd_query", "fa_fwd_reference_bias", "fa_strerror",
-           "fa_fwd_timed", "fa_fwd_timed_ex", "fa_qkv_proj", "fa_qkv_proj_plan", "fa_qkv_proj_variant")
+           "fa_fwd_timed", "fa_fwd_timed_ex", "fa_qkv_proj", "fa_qkv_proj_plan", "fa_qkv_proj_variant",
+           "fa_cache_append", "fa_cached_attention", "fa_cached_attention_workspace", "fa_select_pages", "fa_select_pages_workspace")
 FLAG_CAUSAL = 1
 FLAG_BF16 = 2
 
 _lib = None
+
+
+class Cache(ctypes.Structure):
+    """fa_cache: addresses and sizes of a paged key/value cache and its page table."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("keys", "values", "key_exponents", "value_exponents", "key_bounds", "page_table")] +
+                [(name, ctypes.c_int64) for name in ("pages", "heads", "page_size", "head_dim", "sequences", "table_width", "table_stride")])
 
 
 class FusedAttnError(RuntimeError):
@@ -66,6 +74,19 @@ def load_library():
     lib.fa_fwd_query.restype = ctypes.c_int
     lib.fa_fwd_reference_bias.argtypes = [i64]
     lib.fa_fwd_reference_bias.restype = f32
+    cache = ctypes.POINTER(Cache)
+    lib.fa_cache_append.argtypes = [cache, vp, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, i64, i64, vp, vp, i64,
+                                    ctypes.c_int, vp]
+    lib.fa_cache_append.restype = ctypes.c_int
+    lib.fa_cached_attention.argtypes = [cache, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, i64, vp, vp, i64, i64, f32, ctypes.c_int,
+                                        vp, i64, vp]
+    lib.fa_cached_attention.restype = ctypes.c_int
+    lib.fa_cached_attention_workspace.argtypes = [cache, i64, i64, i64]
+    lib.fa_cached_attention_workspace.restype = i64
+    lib.fa_select_pages.argtypes = [cache, vp, i64, i64, i64, vp, i64, vp, vp, i64, i64, ctypes.c_int, vp, i64, vp]
+    lib.fa_select_pages.restype = ctypes.c_int
+    lib.fa_select_pages_workspace.argtypes = [cache, i64, i64]
+    lib.fa_select_pages_workspace.restype = i64
     lib.fa_strerror.argtypes = [ctypes.c_int]
     lib.fa_strerror.restype = ctypes.c_char_p
     _lib = lib
@@ -317,3 +338,199 @@ def qkv_project(x, w, num_heads, head_dim, bias=None, rope=None, out=None):
             tables[1].data_ptr() if rope is not None else None, flags, _current_stream(x) or None)
     _check(status)
     return out
+
+
+def _kind(name, t, dtype, shape=None, contiguous=True):
+    import torch
+
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    if t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, list(shape), tuple(t.shape)))
+    if contiguous and not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return t
+
+
+def _cache(k_exponents, page_table, starts, new_lens, page_size, head_dim, k_cache=None, v_cache=None, v_exponents=None,
+           key_bounds=None):
+    """The fa_cache of checked tensors, and the tensors."""
+    import torch
+
+    _kind("k_exponents", k_exponents, torch.int8)
+    if k_exponents.dim() != 2 or k_exponents.numel() == 0:
+        raise ValueError("k_exponents must be [pages, key heads], got %s" % (tuple(k_exponents.shape),))
+    pages, heads = k_exponents.shape
+    if head_dim not in (16, 32, 64, 128):
+        raise ValueError("head_dim must be 16, 32, 64 or 128, got %r" % (head_dim,))
+    if page_size not in (16, 32, 64, 128):
+        raise ValueError("the pages must hold 16, 32, 64 or 128 tokens, got %r" % (page_size,))
+    _kind("page_table", page_table, torch.int32, contiguous=False)
+    if page_table.dim() != 2 or page_table.numel() == 0 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must be [batch, width] with dense rows, got %s" % (tuple(page_table.shape),))
+    B, W = page_table.shape
+    tensors = [k_exponents, page_table, _kind("starts", starts, torch.int32, (B,))]
+    if new_lens is not None:
+        tensors.append(_kind("new_lens", new_lens, torch.int32, (B,)))
+    c = Cache(key_exponents=k_exponents.data_ptr(), page_table=page_table.data_ptr(), pages=pages, heads=heads, page_size=page_size,
+              head_dim=head_dim, sequences=B, table_width=W, table_stride=page_table.stride(0) if B > 1 else W)
+    if k_cache is not None:
+        shape = (pages, heads, page_size, head_dim)
+        c.keys = _kind("k_cache", k_cache, torch.float8_e4m3fn, shape).data_ptr()
+        c.values = _kind("v_cache", v_cache, torch.float8_e4m3fn, shape).data_ptr()
+        c.value_exponents = _kind("v_exponents", v_exponents, torch.int8, (pages, heads)).data_ptr()
+        tensors += [k_cache, v_cache, v_exponents]
+    if key_bounds is not None:
+        c.key_bounds = _kind("key_bounds", key_bounds, torch.int8, (pages, heads, 2, head_dim)).data_ptr()
+        tensors.append(key_bounds)
+    return c, tensors
+
+
+def _tokens(name, t, layout, c):
+    """(L, heads, (stride_b, stride_h, stride_l)) of new tokens; the strides of dimensions of one element, which mean nothing,
+    as the library takes them."""
+    import torch
+
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    if t.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("%s must be float16 or bfloat16, got %s" % (name, t.dtype))
+    if layout not in ("blf", "bhld"):
+        raise ValueError("layout must be 'blf' or 'bhld'")
+    if t.dim() != (3 if layout == "blf" else 4):
+        raise ValueError("layout %r takes %d-D tensors, %s has %d dimensions" % (layout, 3 if layout == "blf" else 4, name, t.dim()))
+    if min(t.shape) < 1:
+        raise ValueError("%s must not have an empty dimension, got %s" % (name, tuple(t.shape)))
+    if t.shape[0] != c.sequences:
+        raise ValueError("%s must have the batch of page_table (%d), got %s" % (name, c.sequences, tuple(t.shape)))
+    if layout == "blf" and t.shape[2] % c.head_dim != 0:
+        raise ValueError("the features of %s (%d) must be a multiple of head_dim (%d)" % (name, t.shape[2], c.head_dim))
+    if layout == "bhld" and t.shape[3] != c.head_dim:
+        raise ValueError("the last dimension of %s (%d) must equal head_dim (%d)" % (name, t.shape[3], c.head_dim))
+    L, heads = (t.shape[1], t.shape[2] // c.head_dim) if layout == "blf" else (t.shape[2], t.shape[1])
+    sb, sh, sl = _strides(t, c.head_dim, layout, name)
+    return L, heads, (sb if c.sequences > 1 else 0, sh if heads > 1 else 0, sl if L > 1 else c.head_dim)
+
+
+def _on_one_gpu(tensors):
+    """Last, so that the checks before it can be exercised on host tensors."""
+    for t in tensors:
+        if not t.is_cuda or t.device != tensors[0].device:
+            raise ValueError("all tensors must be on one GPU, got devices %s and %s" % (tensors[0].device, t.device))
+
+
+def _query_tokens(queries, out, layout, c):
+    L, R, strides = _tokens("queries", queries, layout, c)
+    if R % c.heads != 0:
+        raise ValueError("the heads of queries (%d) must be a multiple of the key heads (%d)" % (R, c.heads))
+    if out is not None and (out.shape != queries.shape or out.dtype != queries.dtype):
+        raise ValueError("out must have the shape and dtype of queries")
+    return L, R, strides
+
+
+def cache_append(keys, values, k_cache, v_cache, k_exponents, v_exponents, page_table, starts, new_lens=None, queries=None,
+                 rope=None, key_bounds=None, layout="blf", out=None):
+    """fa_cache_append on torch GPU tensors, on torch's current stream: appends keys (rotated by rope = (cos, sin), float32
+    [positions, head_dim / 2] tables) and values to the cache in place.  Returns the rotated queries (`out`, allocated when not
+    given), or None without queries.  The cache's tensors are described in include/fused_attn.h."""
+    import torch
+
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be [pages, key heads, page_size, head_dim], got %s" % (tuple(k_cache.shape),))
+    c, tensors = _cache(k_exponents, page_table, starts, new_lens, k_cache.shape[2], k_cache.shape[3], k_cache, v_cache, v_exponents,
+                        key_bounds)
+    L, heads, kv = _tokens("keys", keys, layout, c)
+    if heads != c.heads:
+        raise ValueError("keys must have the key heads of the cache (%d), got %d" % (c.heads, heads))
+    if values.dtype != keys.dtype or values.shape != keys.shape or _tokens("values", values, layout, c)[2] != kv:
+        raise ValueError("values must have the dtype, shape and strides of keys")
+    R, q, o = c.heads, (0, 0, 0), (0, 0, 0)
+    if queries is None and out is not None:
+        raise ValueError("out goes with queries")
+    if queries is not None:
+        Lq, R, q = _query_tokens(queries, out, layout, c)
+        if Lq != L or queries.dtype != keys.dtype:
+            raise ValueError("queries must have the seq_len and dtype of keys")
+        out = torch.empty(queries.shape, dtype=queries.dtype, device=queries.device) if out is None else out
+        o = _tokens("out", out, layout, c)[2]
+    tables = (None, None)
+    if rope is not None:
+        if isinstance(rope, torch.Tensor) or not isinstance(rope, (tuple, list)) or len(rope) != 2:
+            raise ValueError("rope must be a pair (cos, sin) of float32 [positions, head_dim / 2] tensors")
+        tables = tuple(rope)
+        for name, t in zip(("rope cos", "rope sin"), tables):
+            _kind(name, t, torch.float32, (tables[0].shape[0], c.head_dim // 2))
+    _on_one_gpu(tensors + [keys, values] + [t for t in (queries, out) + tables if t is not None])
+    with torch.cuda.device(keys.device):
+        _check(load_library().fa_cache_append(
+            ctypes.byref(c), keys.data_ptr(), values.data_ptr(), *kv, queries.data_ptr() if queries is not None else None, *q,
+            out.data_ptr() if queries is not None else None, *o, starts.data_ptr(),
+            new_lens.data_ptr() if new_lens is not None else None, L, R, tables[0].data_ptr() if rope is not None else None,
+            tables[1].data_ptr() if rope is not None else None, tables[0].shape[0] if rope is not None else 0,
+            FLAG_BF16 if keys.dtype == torch.bfloat16 else 0, _current_stream(keys) or None))
+    return out
+
+
+def _bytes(status):
+    if status < 0:
+        _check(int(status))
+    return status
+
+
+def cached_attention(queries, k_cache, v_cache, k_exponents, v_exponents, page_table, starts, new_lens=None, pages=None, causal=True,
+                     return_lse=False, layout="blf", scale=None, out=None):
+    """fa_cached_attention on torch GPU tensors, on torch's current stream: attention of new tokens over the cache, or over the
+    pages that `pages`, int32 [batch, seq_len, key heads, count], lists.  Returns `out` (allocated when not given), or
+    (out, lse)."""
+    import torch
+
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be [pages, key heads, page_size, head_dim], got %s" % (tuple(k_cache.shape),))
+    c, tensors = _cache(k_exponents, page_table, starts, new_lens, k_cache.shape[2], k_cache.shape[3], k_cache, v_cache, v_exponents)
+    L, R, q = _query_tokens(queries, out, layout, c)
+    count = 0
+    if pages is not None:
+        _kind("pages", pages, torch.int32)
+        if pages.dim() != 4 or tuple(pages.shape[:3]) != (c.sequences, L, c.heads) or pages.shape[3] < 1:
+            raise ValueError("pages must be [batch, seq_len, key heads, count], got %s" % (tuple(pages.shape),))
+        count = pages.shape[3]
+    out = torch.empty(queries.shape, dtype=queries.dtype, device=queries.device) if out is None else out
+    o = _tokens("out", out, layout, c)[2]
+    _on_one_gpu(tensors + [queries, out] + ([pages] if pages is not None else []))
+    lib = load_library()
+    lse = torch.empty((c.sequences, R, L), dtype=torch.float32, device=queries.device) if return_lse else None
+    nbytes = _bytes(lib.fa_cached_attention_workspace(ctypes.byref(c), L, R, count))
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=queries.device) if nbytes else None
+    flags = (FLAG_CAUSAL if causal else 0) | (FLAG_BF16 if queries.dtype == torch.bfloat16 else 0)
+    with torch.cuda.device(queries.device):
+        _check(lib.fa_cached_attention(
+            ctypes.byref(c), queries.data_ptr(), *q, out.data_ptr(), *o, lse.data_ptr() if return_lse else None,
+            pages.data_ptr() if pages is not None else None, count, starts.data_ptr(),
+            new_lens.data_ptr() if new_lens is not None else None, L, R, 1.0 / math.sqrt(c.head_dim) if scale is None else scale, flags,
+            workspace.data_ptr() if nbytes else None, nbytes, _current_stream(queries) or None))
+    return (out, lse) if return_lse else out
+
+
+def select_pages(queries, key_bounds, k_exponents, page_table, starts, page_size, count, new_lens=None, layout="blf"):
+    """fa_select_pages on torch GPU tensors, on torch's current stream.  Returns int32 [batch, seq_len, key heads, count]."""
+    import torch
+
+    if key_bounds.dim() != 4:
+        raise ValueError("key_bounds must be [pages, key heads, 2, head_dim], got %s" % (tuple(key_bounds.shape),))
+    c, tensors = _cache(k_exponents, page_table, starts, new_lens, page_size, key_bounds.shape[3], key_bounds=key_bounds)
+    L, R, q = _query_tokens(queries, None, layout, c)
+    if int(count) != count or count < 1:
+        raise ValueError("count must be a positive integer, got %r" % (count,))
+    _on_one_gpu(tensors + [queries])
+    lib = load_library()
+    nbytes = _bytes(lib.fa_select_pages_workspace(ctypes.byref(c), L, R))
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=queries.device) if nbytes else None
+    selected = torch.empty((c.sequences, L, c.heads, count), dtype=torch.int32, device=queries.device)
+    with torch.cuda.device(queries.device):
+        _check(lib.fa_select_pages(
+            ctypes.byref(c), queries.data_ptr(), *q, selected.data_ptr(), count, starts.data_ptr(),
+            new_lens.data_ptr() if new_lens is not None else None, L, R, FLAG_BF16 if queries.dtype == torch.bfloat16 else 0,
+            workspace.data_ptr() if nbytes else None, nbytes, _current_stream(queries) or None))
+    return selected

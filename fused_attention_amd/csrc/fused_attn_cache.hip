@@ -1,0 +1,301 @@
+// C ABI of the paged key/value cache (include/fused_attn.h): argument validation, the choice of launch and the launches.
+// A translation unit of its own, so that the attention and projection kernels are compiled as they were.
+#include "cache_kernels.hpp"
+
+#include "../../include/fused_attn.h"
+
+#include <mutex>
+#include <utility>
+#include <vector>
+
+namespace {
+
+using fa::cache::AppendParams;
+using fa::cache::AttendParams;
+using fa::cache::SelectParams;
+using fa::cache::Strides3;
+using fa::cache::View;
+
+constexpr int kNumCu = 256;
+constexpr int64_t kMaxInt = 0x7fffffff - 0x10000;
+constexpr int64_t kMaxElems = (int64_t)1 << 62;
+constexpr int64_t kMostThreads = 0xffffffffll;       // of a grid: the dispatch packet holds no more
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+bool below(int64_t a, int64_t b, int64_t most) { return a <= most / b; }     // a * b <= most, for positive b
+
+// The sizes of the cache and the call, without any pointer.
+int check_sizes(const fa_cache* c, int64_t L, int64_t R, View* p) {
+    if (c == nullptr) return FA_ERR_NULL_POINTER;
+    if (!fa_fwd_query(c->head_dim)) return FA_ERR_BAD_HEAD_DIM;
+    int log2_p = 4;
+    while (log2_p < 7 && ((int64_t)1 << log2_p) < c->page_size) ++log2_p;
+    if (c->page_size != (int64_t)1 << log2_p) return FA_ERR_BAD_PAGE;
+    if (c->pages < 1 || c->heads < 1 || c->sequences < 1 || c->table_width < 1 || L < 1 || R < 1 || R % c->heads != 0) return FA_ERR_BAD_SHAPE;
+    if (c->table_stride < c->table_width && c->sequences > 1) return FA_ERR_BAD_STRIDE;
+    if (c->table_stride < 0) return FA_ERR_BAD_STRIDE;
+    if (c->pages > kMaxInt || c->heads > kMaxInt || R > kMaxInt || L > kMaxInt || c->sequences > kMaxInt || c->table_width > kMaxInt)
+        return FA_ERR_TOO_LARGE;
+    if (!below(c->pages * c->heads, c->page_size / 16, kMaxInt) || !below(c->table_width, c->page_size, kMaxInt) ||
+        !below(L, R, kMaxInt) || !below(L * R, c->sequences, kMaxInt) || !below(c->table_stride, c->sequences, kMaxElems))
+        return FA_ERR_TOO_LARGE;
+    p->k = static_cast<uint8_t*>(c->keys);
+    p->v = static_cast<uint8_t*>(c->values);
+    p->k_exponents = static_cast<int8_t*>(c->key_exponents);
+    p->v_exponents = static_cast<int8_t*>(c->value_exponents);
+    p->bounds = static_cast<int8_t*>(c->key_bounds);
+    p->table = c->page_table;
+    p->table_stride = c->table_stride;
+    p->B = (int)c->sequences;
+    p->L = (int)L;
+    p->R = (int)R;
+    p->Rkv = (int)c->heads;
+    p->W = (int)c->table_width;
+    p->pages = (int)c->pages;
+    p->log2_p = log2_p;
+    p->group = (int)(R / c->heads);
+    return FA_OK;
+}
+
+int check_tensors(const fa_cache* c, const int32_t* starts, const int32_t* new_lens, bool values, View* p) {
+    if (starts == nullptr || c->page_table == nullptr || c->key_exponents == nullptr) return FA_ERR_NULL_POINTER;
+    if (values && (c->keys == nullptr || c->values == nullptr || c->value_exponents == nullptr)) return FA_ERR_NULL_POINTER;
+    if (!aligned(starts, 4) || !aligned(new_lens, 4) || !aligned(c->page_table, 4)) return FA_ERR_MISALIGNED;
+    if (!aligned(c->key_bounds, 16) || (values && (!aligned(c->keys, 16) || !aligned(c->values, 16)))) return FA_ERR_MISALIGNED;
+    p->starts = starts;
+    p->new_lens = new_lens;
+    return FA_OK;
+}
+
+// A tensor under the addressing rule: its strides, alignment and extent.
+int check_strided(const void* t, const Strides3& s, int64_t B, int64_t heads, int64_t L, int64_t H) {
+    if (t == nullptr) return FA_ERR_NULL_POINTER;
+    if (s.b < 0 || s.h < 0 || s.l < H || s.b % 8 != 0 || s.h % 8 != 0 || s.l % 8 != 0) return FA_ERR_BAD_STRIDE;
+    if (!aligned(t, 16)) return FA_ERR_MISALIGNED;
+    if (!below(L, s.l, kMaxElems) || (s.h > 0 && !below(heads, s.h, kMaxElems)) || (s.b > 0 && !below(B, s.b, kMaxElems))) return FA_ERR_TOO_LARGE;
+    return FA_OK;
+}
+
+// Dynamic LDS above 64 KiB has to be opted into per kernel function and per device.
+hipError_t allow_large_lds(const void* kernel, int bytes) {
+    static std::mutex lock;
+    static std::vector<std::pair<const void*, int>> done;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    std::lock_guard<std::mutex> guard(lock);
+    for (const auto& d : done)
+        if (d.first == kernel && d.second == dev) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.emplace_back(kernel, dev);
+    return e;
+}
+
+template <class Params>
+hipError_t launch(void (*kernel)(const Params), int64_t wgs, int threads, const Params& p, int lds, hipStream_t stream) {
+    Params params = p;
+    void* args[] = {&params};
+    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((uint32_t)wgs), dim3(threads), args, lds, stream);
+}
+
+// f(std::integral_constant<int, H>, std::bool_constant<BF>) for a run-time head_dim and type
+template <class F>
+hipError_t for_type(int64_t H, bool bf, F f) {
+    auto with = [&](auto h) { return bf ? f(h, std::true_type{}) : f(h, std::false_type{}); };
+    switch (H) {
+        case 16: return with(std::integral_constant<int, 16>{});
+        case 32: return with(std::integral_constant<int, 32>{});
+        case 64: return with(std::integral_constant<int, 64>{});
+        default: return with(std::integral_constant<int, 128>{});
+    }
+}
+
+// How cached_attention is launched.
+struct AttendPlan {
+    int nq;                // blocks of 16 query rows of a workgroup
+    int64_t tiles, splits, wgs;
+};
+
+AttendPlan plan_attend(const View& p, int64_t count) {
+    AttendPlan a;
+    const int64_t rows = (int64_t)p.L * p.group;
+    a.nq = count > 0 || rows <= 16 ? 1 : 2;
+    a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, 16 * a.nq);
+    const int64_t base = (int64_t)p.B * p.Rkv * a.tiles;
+    // two workgroups for each compute unit, and a step of 64 tokens at least for each wave
+    const int64_t most_keys = (count > 0 ? count : (int64_t)p.W) << p.log2_p;
+    const int64_t most = ceil_div(most_keys, 64 * fa::cache::kAttendWaves);
+    a.splits = ceil_div(2 * kNumCu, base);
+    if (a.splits > most) a.splits = most;
+    if (a.splits > 64) a.splits = 64;
+    a.wgs = base * a.splits;
+    return a;
+}
+
+int64_t attend_workspace(const View& p, const AttendPlan& a, int64_t H) {
+    return a.splits > 1 ? (int64_t)p.B * p.L * p.R * a.splits * (H + 1) * 4 : 0;
+}
+
+int check_count(int64_t count) { return count > fa::cache::kMostSelected ? FA_ERR_TOO_LARGE : FA_OK; }
+
+constexpr int kMostTable = 32768;
+
+}  // namespace
+
+extern "C" {
+
+int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t kv_stride_b, int64_t kv_stride_h, int64_t kv_stride_l,
+                    const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, void* q_out, int64_t out_stride_b,
+                    int64_t out_stride_h, int64_t out_stride_l, const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R,
+                    const float* rope_cos, const float* rope_sin, int64_t rope_rows, int flags, void* stream) {
+    if ((flags & ~FA_FLAG_BF16) != 0) return FA_ERR_BAD_FLAGS;
+    AppendParams p;
+    int rc = check_sizes(cache, L, q != nullptr || cache == nullptr ? R : cache->heads, &p);
+    if (rc == FA_OK) rc = check_tensors(cache, starts, new_lens, true, &p);
+    if (rc != FA_OK) return rc;
+    const int64_t B = cache->sequences, H = cache->head_dim;
+    p.kv = {kv_stride_b, kv_stride_h, kv_stride_l};
+    p.qs = {q_stride_b, q_stride_h, q_stride_l};
+    p.qo = {out_stride_b, out_stride_h, out_stride_l};
+    for (const void* t : {k, v})
+        if ((rc = check_strided(t, p.kv, B, cache->heads, L, H)) != FA_OK) return rc;
+    if ((q == nullptr) != (q_out == nullptr)) return FA_ERR_NULL_POINTER;
+    if (q != nullptr && (rc = check_strided(q, p.qs, B, R, L, H)) != FA_OK) return rc;
+    if (q != nullptr && (rc = check_strided(q_out, p.qo, B, R, L, H)) != FA_OK) return rc;
+    if ((rope_cos == nullptr) != (rope_sin == nullptr)) return FA_ERR_NULL_POINTER;
+    if (rope_cos != nullptr && rope_rows < 1) return FA_ERR_BAD_SHAPE;
+    if (!aligned(rope_cos, 16) || !aligned(rope_sin, 16)) return FA_ERR_MISALIGNED;
+    p.key = static_cast<const uint16_t*>(k);
+    p.value = static_cast<const uint16_t*>(v);
+    p.q = static_cast<const uint16_t*>(q);
+    p.q_out = static_cast<uint16_t*>(q_out);
+    p.rope_cos = rope_cos;
+    p.rope_sin = rope_sin;
+    p.rope_rows = rope_rows;
+    const int64_t P = cache->page_size;
+    // the page of the first token, and those of the others
+    const int64_t reach = (L + P - 2) / P + 1;
+    p.reach = (int)(reach < p.W ? reach : p.W);
+    p.cache_items = B * p.reach * cache->heads * 2;
+    p.q_units = q != nullptr ? B * L * R * (H / 16) : 0;
+    const bool bf = (flags & FA_FLAG_BF16) != 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t units = (L < P ? L : P) * (H / 16);    // of a page's new tokens
+    const int threads = units <= 64 ? 64 : 256;
+    const int64_t wgs = p.cache_items + ceil_div(p.q_units, threads);
+    if (wgs > kMostThreads / threads || p.cache_items > 0x7fffffff) return FA_ERR_TOO_LARGE;
+    return static_cast<int>(for_type(H, bf, [&](auto h, auto b) {
+        using namespace fa::cache;
+        if (units <= 64) return launch(cache_append_kernel<h(), b(), 64, 1>, wgs, 64, p, 0, s);
+        if constexpr (h() >= 128)
+            if (units > 512) return launch(cache_append_kernel<h(), b(), 256, 4>, wgs, 256, p, 0, s);
+        if constexpr (h() >= 64)
+            if (units > 256) return launch(cache_append_kernel<h(), b(), 256, 2>, wgs, 256, p, 0, s);
+        return launch(cache_append_kernel<h(), b(), 256, 1>, wgs, 256, p, 0, s);
+    }));
+}
+
+int64_t fa_cached_attention_workspace(const fa_cache* cache, int64_t L, int64_t R, int64_t count) {
+    View p;
+    int rc = check_sizes(cache, L, R, &p);
+    if (rc == FA_OK) rc = check_count(count);
+    if (rc == FA_OK && count < 0) rc = FA_ERR_BAD_SHAPE;
+    if (rc != FA_OK) return rc;
+    return attend_workspace(p, plan_attend(p, count), cache->head_dim);
+}
+
+int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, void* out,
+                        int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, void* lse, const int32_t* selected,
+                        int64_t count, const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R, float scale, int flags,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+    if ((flags & ~(FA_FLAG_BF16 | FA_FLAG_CAUSAL)) != 0) return FA_ERR_BAD_FLAGS;
+    AttendParams p;
+    int rc = check_sizes(cache, L, R, &p);
+    if (rc == FA_OK) rc = check_tensors(cache, starts, new_lens, true, &p);
+    if (rc != FA_OK) return rc;
+    if (selected != nullptr && count < 1) return FA_ERR_BAD_SHAPE;
+    if (selected == nullptr) count = 0;
+    if ((rc = check_count(count)) != FA_OK) return rc;
+    if (!(scale > 0.f) || scale > 3.0e38f) return FA_ERR_BAD_SCALE;
+    const int64_t B = cache->sequences, H = cache->head_dim;
+    p.qs = {q_stride_b, q_stride_h, q_stride_l};
+    p.os = {out_stride_b, out_stride_h, out_stride_l};
+    if ((rc = check_strided(q, p.qs, B, R, L, H)) != FA_OK) return rc;
+    if ((rc = check_strided(out, p.os, B, R, L, H)) != FA_OK) return rc;
+    if (!aligned(lse, 4) || !aligned(selected, 4)) return FA_ERR_MISALIGNED;
+    const AttendPlan a = plan_attend(p, count);
+    if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * fa::cache::kAttendWaves)) return FA_ERR_TOO_LARGE;
+    const int64_t need = attend_workspace(p, a, H);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FA_ERR_WORKSPACE;
+    if (need > 0 && !aligned(workspace, 16)) return FA_ERR_MISALIGNED;
+    p.q = static_cast<const uint16_t*>(q);
+    p.out = static_cast<uint16_t*>(out);
+    p.lse = static_cast<float*>(lse);
+    p.selected = selected;
+    p.count = (int)count;
+    p.causal = (flags & FA_FLAG_CAUSAL) != 0;
+    p.tiles = (int)a.tiles;
+    p.splits = (int)a.splits;
+    p.total_wgs = (int)a.wgs;
+    p.wgs_per_xcd = (int)ceil_div(a.wgs, fa::kNumXcd);
+    p.scale_log2e = scale * 1.4426950408889634f;
+    const int64_t rows = B * L * R;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = p.part_o + rows * a.splits * H;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t grid = (int64_t)p.wgs_per_xcd * fa::kNumXcd;
+    return static_cast<int>(for_type(H, (flags & FA_FLAG_BF16) != 0, [&](auto h, auto b) {
+        using namespace fa::cache;
+        constexpr int threads = 64 * kAttendWaves;
+        hipError_t e;
+        if (count > 0)
+            e = launch(cached_attention_kernel<h(), b(), 1, true>, grid, threads, p, 0, s);
+        else if (a.nq == 1)
+            e = launch(cached_attention_kernel<h(), b(), 1, false>, grid, threads, p, 0, s);
+        else
+            e = launch(cached_attention_kernel<h(), b(), 2, false>, grid, threads, p, 0, s);
+        if (e != hipSuccess || a.splits == 1) return e;
+        return launch(cached_attention_join_kernel<h(), b()>, ceil_div(rows * (h() / 8), 256), 256, p, 0, s);
+    }));
+}
+
+int64_t fa_select_pages_workspace(const fa_cache* cache, int64_t L, int64_t R) {
+    View p;
+    const int rc = check_sizes(cache, L, R, &p);
+    if (rc != FA_OK) return rc;
+    if (p.W > kMostTable) return FA_ERR_TOO_LARGE;
+    return 0;
+}
+
+int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, int32_t* selected,
+                    int64_t count, const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R, int flags, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+    if ((flags & ~FA_FLAG_BF16) != 0) return FA_ERR_BAD_FLAGS;
+    SelectParams p;
+    int rc = check_sizes(cache, L, R, &p);
+    if (rc == FA_OK) rc = check_tensors(cache, starts, new_lens, false, &p);
+    if (rc != FA_OK) return rc;
+    if (selected == nullptr || cache->key_bounds == nullptr) return FA_ERR_NULL_POINTER;
+    if (count < 1) return FA_ERR_BAD_SHAPE;
+    if (p.W > kMostTable || (rc = check_count(count)) != FA_OK) return FA_ERR_TOO_LARGE;
+    p.qs = {q_stride_b, q_stride_h, q_stride_l};
+    if ((rc = check_strided(q, p.qs, p.B, R, L, cache->head_dim)) != FA_OK) return rc;
+    if (!aligned(selected, 4)) return FA_ERR_MISALIGNED;
+    p.q = static_cast<const uint16_t*>(q);
+    p.selected = selected;
+    p.count = (int)count;
+    (void)workspace;
+    (void)workspace_bytes;
+    const int64_t wgs = (int64_t)p.B * L * p.Rkv;
+    if (wgs > kMostThreads / fa::cache::kSelectThreads) return FA_ERR_TOO_LARGE;
+    return static_cast<int>(for_type(cache->head_dim, (flags & FA_FLAG_BF16) != 0, [&](auto h, auto b) {
+        using namespace fa::cache;
+        auto kernel = select_pages_kernel<h(), b()>;
+        const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), kMostTable * 4);
+        if (e != hipSuccess) return e;
+        return launch(kernel, wgs, kSelectThreads, p, p.W * 4, static_cast<hipStream_t>(stream));
+    }));
+}
+
+}  // extern "C"

@@ -626,16 +626,18 @@ float fa_fwd_reference_bias(int64_t L) {
 const char* fa_strerror(int status) {
     switch (status) {
         case FA_OK: return "success";
-        case FA_ERR_NULL_POINTER: return "fa_fwd: q, k, v and out must be non-null device pointers";
+        case FA_ERR_NULL_POINTER: return "fa_fwd: q, k, v and out must be non-null device pointers (fa_cache: and all that is not nullable)";
         case FA_ERR_BAD_HEAD_DIM: return "fa_fwd: head_dim must be 16, 32, 64 or 128";
         case FA_ERR_BAD_SHAPE:
-            return "fa_fwd: B, R and L must be at least 1 (fa_qkv_proj: and the feature counts multiples of 64)";
+            return "fa_fwd: B, R and L must be at least 1 (fa_qkv_proj: and the feature counts multiples of 64; fa_cache: and every size, R a multiple of heads)";
         case FA_ERR_BAD_STRIDE:
             return "fa_fwd: strides must be non-negative multiples of 8 elements and stride_l >= head_dim";
-        case FA_ERR_MISALIGNED: return "fa_fwd: q, k, v and out must be 16-byte aligned";
+        case FA_ERR_MISALIGNED: return "fa_fwd: q, k, v and out must be 16-byte aligned (fa_cache: and keys, values, key_bounds, rope tables and workspace)";
         case FA_ERR_TOO_LARGE: return "fa_fwd: problem size exceeds the supported index range";
         case FA_ERR_BAD_FLAGS: return "fa_fwd_ex: unknown flag, or FA_FLAG_CAUSAL together with a mask";
         case FA_ERR_BAD_SCALE: return "fa_fwd: scale must be finite and positive";
+        case FA_ERR_BAD_PAGE: return "fa_cache: page_size must be 16, 32, 64 or 128";
+        case FA_ERR_WORKSPACE: return "fa_cached_attention, fa_select_pages: the workspace is smaller than their _workspace functions say";
         default: break;
     }
     if (status > 0) return hipGetErrorString(static_cast<hipError_t>(status));

@@ -271,6 +271,8 @@ torch::Tensor qkv_projection(torch::Tensor hidden, torch::Tensor weight, std::op
     return qkv;
 }
 
+#include "fused_attn_cache_binding.inc"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -295,4 +297,31 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("bias") = std::optional<torch::Tensor>(), py::arg("num_heads"), py::arg("head_dim"),
           py::arg("rope_cos") = std::optional<torch::Tensor>(), py::arg("rope_sin") = std::optional<torch::Tensor>(),
           "Fused QKV projection into the packed [batch, seq_len, 3, num_heads * head_dim] tensor");
+    m.def("cache_append", &cache_append, py::arg("keys"), py::arg("values"), py::arg("k_cache"), py::arg("v_cache"),
+          py::arg("k_exponents"), py::arg("v_exponents"), py::arg("page_table"), py::arg("starts"),
+          py::arg("new_lens") = std::optional<torch::Tensor>(), py::arg("queries") = std::optional<torch::Tensor>(),
+          py::arg("rope_cos") = std::optional<torch::Tensor>(), py::arg("rope_sin") = std::optional<torch::Tensor>(),
+          py::arg("key_bounds") = std::optional<torch::Tensor>(), py::arg("layout") = "blf",
+          "Appends keys (rotated by their positions) and values to a paged 8-bit cache, in place.  Returns the rotated queries, "
+          "or None without queries.");
+    m.def("cached_attention",
+          [](torch::Tensor queries, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_exponents, torch::Tensor v_exponents,
+             torch::Tensor page_table, torch::Tensor starts, std::optional<torch::Tensor> new_lens, std::optional<torch::Tensor> pages,
+             bool causal, bool return_lse, const std::string& layout, std::optional<double> scale) -> py::object {
+              const std::vector<torch::Tensor> r = cached_attention(queries, k_cache, v_cache, k_exponents, v_exponents, page_table,
+                                                                    starts, new_lens, pages, causal, return_lse, layout, scale);
+              if (r.size() == 1) return py::cast(r[0]);
+              return py::make_tuple(r[0], r[1]);
+          },
+          py::arg("queries"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_exponents"), py::arg("v_exponents"),
+          py::arg("page_table"), py::arg("starts"), py::arg("new_lens") = std::optional<torch::Tensor>(),
+          py::arg("pages") = std::optional<torch::Tensor>(), py::arg("causal") = true, py::arg("return_lse") = false,
+          py::arg("layout") = "blf", py::arg("scale") = std::optional<double>(),
+          "Multihead attention of new tokens over a paged 8-bit cache, or over those of its pages that `pages` lists for each "
+          "token and key head.  Returns output, or (output, lse).");
+    m.def("select_pages", &select_pages, py::arg("queries"), py::arg("key_bounds"), py::arg("k_exponents"), py::arg("page_table"),
+          py::arg("starts"), py::arg("page_size"), py::arg("count"), py::arg("new_lens") = std::optional<torch::Tensor>(),
+          py::arg("layout") = "blf",
+          "The `count` pages whose keys may score highest, for each new token and key head: int32 [batch, seq_len, key heads, "
+          "count], ascending, -1 behind the last.");
 }

@@ -34,6 +34,8 @@ extern "C" {
 #define FA_ERR_TOO_LARGE (-6)
 #define FA_ERR_BAD_FLAGS (-7)
 #define FA_ERR_BAD_SCALE (-8)
+#define FA_ERR_BAD_PAGE (-9)
+#define FA_ERR_WORKSPACE (-10)
 
 #define FA_FLAG_CAUSAL 1
 #define FA_FLAG_BF16 2
@@ -209,6 +211,105 @@ int fa_qkv_proj_plan(int64_t B, int64_t L, int64_t F_in, int64_t R, int64_t H, i
  * per workgroup); workgroups launched; workgroups that do work; output tiles; feature tiles.
  */
 int fa_qkv_proj_variant(int64_t B, int64_t L, int64_t F_in, int64_t R, int64_t H, int rope, int* variant);
+
+/*
+ * A paged cache of keys and values in 8 bits, and the sequences of a call.  No counterpart in the reference, whose keys and
+ * values are the call's own (reference src/fused_attn_extention.cu:15-22): what a program needs that answers token by token.
+ *
+ *   keys, values     [pages, heads, page_size, head_dim], one e4m3 code (OCP FP8: torch.float8_e4m3fn) per value
+ *   key_exponents, value_exponents
+ *                    int8 [pages, heads]: a code c of the page and head stands for c * 2^exponent
+ *   key_bounds       (nullable) int8 [pages, heads, 2, head_dim]: the largest and the smallest key of each channel of the page,
+ *                    in steps of 2^(key exponent + 2), rounded upwards and downwards; what fa_select_pages reads
+ *   page_table       int32 [sequences, table_width], rows table_stride elements apart: the page of the tokens
+ *                    w * page_size .. (w + 1) * page_size - 1 of a sequence; a number outside [0, pages) is no page
+ *
+ * page_size is 16, 32, 64 or 128 (FA_ERR_BAD_PAGE otherwise), head_dim 16, 32, 64 or 128.  All tensors but the table are
+ * contiguous; keys, values and key_bounds 16-byte aligned.  pages * heads * page_size / 16 and
+ * table_width * page_size must stay below 2^31 - 2^16.
+ *
+ * A call brings L tokens for each sequence, of which the first new_lens[b] exist (new_lens NULL: all; numbers outside
+ * [0, L] count as the nearer end); token i of sequence b has the position starts[b] + i, starts[b] being the number of tokens
+ * in the cache before it.  Positions are below table_width * page_size: what lies behind is not written and not read.  starts
+ * and new_lens are int32 [sequences] in device memory.  The library cannot look at numbers in device memory before it
+ * launches; its kernels check every page and every position against the sizes given here, so that wrong ones cost
+ * results, never an access out of bounds.
+ */
+typedef struct fa_cache {
+    void* keys;
+    void* values;
+    void* key_exponents;
+    void* value_exponents;
+    void* key_bounds;
+    const int32_t* page_table;
+    int64_t pages, heads, page_size, head_dim;
+    int64_t sequences, table_width, table_stride;
+} fa_cache;
+
+/*
+ * Appends L new tokens per sequence.  k and v (fp16, or bfloat16 with FA_FLAG_BF16) share (kv_stride_b, kv_stride_h,
+ * kv_stride_l) under the addressing rule above, with cache->heads heads.
+ *   y = k rotated by its position (rotate-half as in fa_qkv_proj, in float32, each product and each sum rounded by itself), where
+ *       rope_cos / rope_sin (both or neither) are float32 [rope_rows, head_dim / 2] tables, indexed by position; v is kept
+ *   e = the smallest exponent, not below -80, with |y| <= 448 * 2^e for all new tokens of the page and head; where the page
+ *       holds earlier tokens of the sequence (its first new token is not in its first place), not below their exponent
+ *   code = e4m3(y * 2^-e), to nearest even; codes of earlier tokens move to e in the same way (without rounding unless they
+ *       become subnormal)
+ * and key_bounds, where the cache has them, follow; they do not depend on the parts in which tokens were appended.  Values that
+ * are not finite become NaN codes and count as zero in the exponent and the bounds.  Tokens at positions from
+ * rope_rows on are not appended; places of a page behind the last token keep their codes, pages that get no token everything.
+ * A page that a call writes must belong to one sequence and stand once in its table.
+ * q (nullable, strides q_stride_*, R heads) is rotated likewise into q_out (strides out_stride_*, not overlapping q),
+ * rounded once; rows of tokens that do not exist, or from rope_rows on, become zeros.  R is not looked at without q.
+ */
+int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t kv_stride_b, int64_t kv_stride_h, int64_t kv_stride_l,
+                    const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,
+                    void* q_out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l,
+                    const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R,
+                    const float* rope_cos, const float* rope_sin, int64_t rope_rows, int flags, void* stream);
+
+/*
+ * out = softmax(q k^T * scale) v over the cached tokens of each sequence, for L tokens of R query heads; R is a multiple of
+ * cache->heads, query head h reads key head h / (R / heads).  Token i of sequence b sees the first starts[b] + i + 1 tokens
+ * with FA_FLAG_CAUSAL (the new ones are in the cache already: fa_cache_append goes first), all starts[b] + new_lens[b]
+ * without, of those on a page; and, where `selected` (nullable) is given, int32 [sequences, L, heads, count], only those on
+ * the pages of its sequence that its list names by their places in the page table, each once however often it is named;
+ * numbers outside [0, table_width) name nothing.  count is at most 4096 (FA_ERR_TOO_LARGE), and not looked at without a list.
+ * Rows that see nothing, and those of tokens that do not exist, are zeros with an lse of -inf.  lse (nullable) as in fa_fwd_ex.
+ * q and out as in fa_fwd_strided, fp16 or bfloat16 (FA_FLAG_BF16), whatever type the cache was filled from.
+ * Accuracy: codes enter both products as they are; scores, sums and outputs are float32; softmax weights are rounded to the
+ * type of q.  fp16 weights keep 11 bits down to 2^-21 of the row's largest, and values 4 bits down to 2^-15 of the largest
+ * power of two among the pages that a wave reads.
+ * A value that is not a number reaches the rows that see it only.
+ * workspace: fa_cached_attention_workspace bytes of device memory, 16-byte aligned (FA_ERR_WORKSPACE if it is too small;
+ * nullable where that is 0), not used by another call at the same time; nothing in it is kept between calls.
+ */
+int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,
+                        void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, void* lse,
+                        const int32_t* selected, int64_t count, const int32_t* starts, const int32_t* new_lens,
+                        int64_t L, int64_t R, float scale, int flags, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that fa_cached_attention needs for these sizes (count = 0: no list), or a negative status.  Only the sizes
+ * in `cache` are looked at; no GPU is touched. */
+int64_t fa_cached_attention_workspace(const fa_cache* cache, int64_t L, int64_t R, int64_t count);
+
+/*
+ * The pages that each new token's query heads attend to: for every token and key head `count` places of the page table in
+ * ascending order into `selected`, int32 [sequences, L, heads, count], -1 behind the last where there are fewer.  Candidates are
+ * the pages up to the one of the token itself, which is always taken; of the others those with the largest
+ *   2^(key exponent) * max over the key head's query heads of  sum_d max(q8_d, 0) * largest_d + min(q8_d, 0) * smallest_d
+ * where q8 = round(q * 2^-e) with the smallest e that keeps the group's queries within 127 (not finite: 0), and largest and
+ * smallest are the cache's key_bounds: an upper bound, up to the rounding of q, of what a key of the page can score.  Whole
+ * numbers throughout; equal scores go to the lowest place.  Tokens that do not exist get -1 only.
+ * q as above, rotated already.  cache->keys, values and value_exponents are not looked at.  table_width is at most 32768
+ * (FA_ERR_TOO_LARGE).  workspace as above, fa_select_pages_workspace bytes.
+ */
+int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,
+                    int32_t* selected, int64_t count, const int32_t* starts, const int32_t* new_lens,
+                    int64_t L, int64_t R, int flags, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that fa_select_pages needs, or a negative status, as above. */
+int64_t fa_select_pages_workspace(const fa_cache* cache, int64_t L, int64_t R);
 
 #ifdef __cplusplus
 }
