@@ -113,20 +113,23 @@ hipError_t for_type(int64_t H, bool bf, F f) {
 
 // How cached_attention is launched.
 struct AttendPlan {
-    int nq;                // blocks of 16 query rows of a workgroup
+    bool wide;             // the kernel for many rows
+    int nq;                // the other one: blocks of 16 query rows of a workgroup
     int64_t tiles, splits, wgs;
 };
 
 AttendPlan plan_attend(const View& p, int64_t count) {
     AttendPlan a;
     const int64_t rows = (int64_t)p.L * p.group;
+    a.wide = count == 0 && rows > 64;
     a.nq = count > 0 || rows <= 16 ? 1 : 2;
-    a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, 16 * a.nq);
+    a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, a.wide ? fa::cache::kWideRows : 16 * a.nq);
     const int64_t base = (int64_t)p.B * p.Rkv * a.tiles;
     // two workgroups for each compute unit, and a step of 64 tokens at least for each wave
     const int64_t most_keys = (count > 0 ? count : (int64_t)p.W) << p.log2_p;
     const int64_t most = ceil_div(most_keys, 64 * fa::cache::kAttendWaves);
-    a.splits = ceil_div(2 * kNumCu, base);
+    a.splits = a.wide ? kNumCu / base : ceil_div(2 * kNumCu, base);
+    if (a.splits < 1) a.splits = 1;
     if (a.splits > most) a.splits = most;
     if (a.splits > 64) a.splits = 64;
     a.wgs = base * a.splits;
@@ -225,7 +228,7 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     if ((rc = check_strided(out, p.os, B, R, L, H)) != FA_OK) return rc;
     if (!aligned(lse, 4) || !aligned(selected, 4)) return FA_ERR_MISALIGNED;
     const AttendPlan a = plan_attend(p, count);
-    if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * fa::cache::kAttendWaves)) return FA_ERR_TOO_LARGE;
+    if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * fa::cache::kWideWaves)) return FA_ERR_TOO_LARGE;
     const int64_t need = attend_workspace(p, a, H);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FA_ERR_WORKSPACE;
     if (need > 0 && !aligned(workspace, 16)) return FA_ERR_MISALIGNED;
@@ -249,7 +252,11 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
         using namespace fa::cache;
         constexpr int threads = 64 * kAttendWaves;
         hipError_t e;
-        if (count > 0)
+        if (a.wide) {
+            auto kernel = cached_attention_wide_kernel<h(), b()>;
+            e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
+            if (e == hipSuccess) e = launch(kernel, grid, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
+        } else if (count > 0)
             e = launch(cached_attention_kernel<h(), b(), 1, true>, grid, threads, p, 0, s);
         else if (a.nq == 1)
             e = launch(cached_attention_kernel<h(), b(), 1, false>, grid, threads, p, 0, s);
