@@ -118,20 +118,42 @@ struct AttendPlan {
     int64_t tiles, splits, wgs;
 };
 
-AttendPlan plan_attend(const View& p, int64_t count) {
+constexpr int64_t kMostSplits = 64;    // the join gives each a lane
+
+// In how many parts the keys of `base` row tiles are cut.  Microseconds, as measured on 14 shapes (up to 64 sequences, 256 to
+// 131072 tokens; every count of parts; the best one is chosen or one within 5 % of it): a wave takes 1 + H / 110 for a step of 64 tokens, or
+// what the bytes of all waves take at 4.8 TB/s where that is more, workgroups beyond one per compute unit in whole rounds;
+// and the second kernel 3.  (B16 Rkv12 H64, 1000 tokens: 9.9 us in one part, 12.8 in two; Rkv8 H128, 2000 tokens: 18.5 in
+// one part, 12.4 in four, 11.4 in eight; 131072 tokens: 75.7 in 16, 58.5 in 32, 66.1 in 48, 60.7 in 64.)
+int64_t pick_splits(int64_t base, int64_t steps, int64_t H) {
+    const float alone = 1.f + 0.009f * (float)H;
+    const float bytes = 0.0273f * (float)H;              // a step of a workgroup's waves, by a 256th of the memory
+    int64_t best = 1;
+    float least = 3.0e38f;
+    for (int64_t s = 1; s <= kMostSplits && (s == 1 || (base * s <= 4 * kNumCu && (s - 1) * fa::cache::kAttendWaves < steps)); ++s) {
+        const int64_t wgs = base * s;
+        const float share = wgs <= kNumCu ? (float)wgs / kNumCu : (float)ceil_div(wgs, kNumCu);
+        const float step = bytes * share > alone ? bytes * share : alone;
+        const float us = step * (float)ceil_div(steps, s * fa::cache::kAttendWaves) + (s > 1 ? 3.f : 0.f);
+        if (us < least) {
+            least = us;
+            best = s;
+        }
+    }
+    return best;
+}
+
+AttendPlan plan_attend(const View& p, int64_t count, int64_t H) {
     AttendPlan a;
     const int64_t rows = (int64_t)p.L * p.group;
     a.wide = count == 0 && rows > 64;
     a.nq = count > 0 || rows <= 16 ? 1 : 2;
     a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, a.wide ? fa::cache::kWideRows : 16 * a.nq);
     const int64_t base = (int64_t)p.B * p.Rkv * a.tiles;
-    // two workgroups for each compute unit, and a step of 64 tokens at least for each wave
-    const int64_t most_keys = (count > 0 ? count : (int64_t)p.W) << p.log2_p;
-    const int64_t most = ceil_div(most_keys, 64 * fa::cache::kAttendWaves);
-    a.splits = a.wide ? kNumCu / base : ceil_div(2 * kNumCu, base);
-    if (a.splits < 1) a.splits = 1;
-    if (a.splits > most) a.splits = most;
-    if (a.splits > 64) a.splits = 64;
+    const int64_t steps = ceil_div((count > 0 ? count : (int64_t)p.W) << p.log2_p, 64);     // of 64 tokens
+    a.splits = a.wide ? (base < kNumCu ? kNumCu / base : 1) : pick_splits(base, steps, H);
+    if (a.splits > kMostSplits) a.splits = kMostSplits;
+    if (a.splits > steps) a.splits = steps;
     a.wgs = base * a.splits;
     return a;
 }
@@ -205,7 +227,7 @@ int64_t fa_cached_attention_workspace(const fa_cache* cache, int64_t L, int64_t 
     if (rc == FA_OK) rc = check_count(count);
     if (rc == FA_OK && count < 0) rc = FA_ERR_BAD_SHAPE;
     if (rc != FA_OK) return rc;
-    return attend_workspace(p, plan_attend(p, count), cache->head_dim);
+    return attend_workspace(p, plan_attend(p, count, cache->head_dim), cache->head_dim);
 }
 
 int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, void* out,
@@ -227,7 +249,7 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     if ((rc = check_strided(q, p.qs, B, R, L, H)) != FA_OK) return rc;
     if ((rc = check_strided(out, p.os, B, R, L, H)) != FA_OK) return rc;
     if (!aligned(lse, 4) || !aligned(selected, 4)) return FA_ERR_MISALIGNED;
-    const AttendPlan a = plan_attend(p, count);
+    const AttendPlan a = plan_attend(p, count, H);
     if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * fa::cache::kWideWaves)) return FA_ERR_TOO_LARGE;
     const int64_t need = attend_workspace(p, a, H);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FA_ERR_WORKSPACE;
@@ -240,14 +262,14 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     p.causal = (flags & FA_FLAG_CAUSAL) != 0;
     p.tiles = (int)a.tiles;
     p.splits = (int)a.splits;
-    p.total_wgs = (int)a.wgs;
-    p.wgs_per_xcd = (int)ceil_div(a.wgs, fa::kNumXcd);
+    p.by_parts = fa::divisor(a.wgs / a.tiles);
+    p.by_splits = fa::divisor(a.splits);
+    p.by_heads = fa::divisor(cache->heads);
     p.scale_log2e = scale * 1.4426950408889634f;
     const int64_t rows = B * L * R;
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + rows * a.splits * H;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t grid = (int64_t)p.wgs_per_xcd * fa::kNumXcd;
     return static_cast<int>(for_type(H, (flags & FA_FLAG_BF16) != 0, [&](auto h, auto b) {
         using namespace fa::cache;
         constexpr int threads = 64 * kAttendWaves;
@@ -255,15 +277,16 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
         if (a.wide) {
             auto kernel = cached_attention_wide_kernel<h(), b()>;
             e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
-            if (e == hipSuccess) e = launch(kernel, grid, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
-        } else if (count > 0)
-            e = launch(cached_attention_kernel<h(), b(), 1, true>, grid, threads, p, 0, s);
-        else if (a.nq == 1)
-            e = launch(cached_attention_kernel<h(), b(), 1, false>, grid, threads, p, 0, s);
-        else
-            e = launch(cached_attention_kernel<h(), b(), 2, false>, grid, threads, p, 0, s);
+            if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
+        } else if (count > 0) {
+            e = launch(cached_attention_kernel<h(), b(), 1, true>, a.wgs, threads, p, 0, s);
+        } else if (a.nq == 1) {
+            e = launch(cached_attention_kernel<h(), b(), 1, false>, a.wgs, threads, p, 0, s);
+        } else {
+            e = launch(cached_attention_kernel<h(), b(), 2, false>, a.wgs, threads, p, 0, s);
+        }
         if (e != hipSuccess || a.splits == 1) return e;
-        return launch(cached_attention_join_kernel<h(), b()>, ceil_div(rows * (h() / 8), 256), 256, p, 0, s);
+        return launch(cached_attention_join_kernel<h(), b()>, ceil_div(rows, 4), 256, p, 0, s);
     }));
 }
 
@@ -294,14 +317,17 @@ int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, in
     p.count = (int)count;
     (void)workspace;
     (void)workspace_bytes;
+    p.by_heads = fa::divisor(p.Rkv);
+    p.by_tokens = fa::divisor(L);
     const int64_t wgs = (int64_t)p.B * L * p.Rkv;
-    if (wgs > kMostThreads / fa::cache::kSelectThreads) return FA_ERR_TOO_LARGE;
+    if (wgs > kMostThreads / 1024) return FA_ERR_TOO_LARGE;
+    const bool many = wgs > 4 * kNumCu;
     return static_cast<int>(for_type(cache->head_dim, (flags & FA_FLAG_BF16) != 0, [&](auto h, auto b) {
         using namespace fa::cache;
-        auto kernel = select_pages_kernel<h(), b()>;
+        auto kernel = many ? select_pages_kernel<h(), b(), 256> : select_pages_kernel<h(), b(), 1024>;
         const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), kMostTable * 4);
         if (e != hipSuccess) return e;
-        return launch(kernel, wgs, kSelectThreads, p, p.W * 4, static_cast<hipStream_t>(stream));
+        return launch(kernel, wgs, many ? 256 : 1024, p, p.W * 4, static_cast<hipStream_t>(stream));
     }));
 }
 
