@@ -114,7 +114,7 @@ hipError_t for_type(int64_t H, bool bf, F f) {
 // How cached_attention is launched.
 struct AttendPlan {
     bool wide;             // the kernel for many rows
-    int nq;                // the other one: blocks of 16 query rows of a workgroup
+    int nq, waves;         // the other one: blocks of 16 query rows and waves of a workgroup
     int64_t tiles, splits, wgs;
 };
 
@@ -150,8 +150,9 @@ AttendPlan plan_attend(const View& p, int64_t count, int64_t H) {
     a.nq = count > 0 || rows <= 16 ? 1 : 2;
     a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, a.wide ? fa::cache::kWideRows : 16 * a.nq);
     const int64_t base = (int64_t)p.B * p.Rkv * a.tiles;
+    a.waves = count > 0 && base > 1000 ? 1 : fa::cache::kAttendWaves;
     const int64_t steps = ceil_div((count > 0 ? count : (int64_t)p.W) << p.log2_p, 64);     // of 64 tokens
-    a.splits = a.wide ? (base < kNumCu ? kNumCu / base : 1) : pick_splits(base, steps, H);
+    a.splits = a.wide ? (base < kNumCu ? kNumCu / base : 1) : a.waves == 1 ? 1 : pick_splits(base, steps, H);
     if (a.splits > kMostSplits) a.splits = kMostSplits;
     if (a.splits > steps) a.splits = steps;
     a.wgs = base * a.splits;
@@ -274,16 +275,18 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
         using namespace fa::cache;
         constexpr int threads = 64 * kAttendWaves;
         hipError_t e;
+        const int list = (int)count * 4;
         if (a.wide) {
             auto kernel = cached_attention_wide_kernel<h(), b()>;
             e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
             if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
         } else if (count > 0) {
-            e = launch(cached_attention_kernel<h(), b(), 1, true>, a.wgs, threads, p, 0, s);
+            e = a.waves == 1 ? launch(cached_attention_kernel<h(), b(), 1, 1, true>, a.wgs, 64, p, list, s)
+                             : launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, true>, a.wgs, threads, p, list, s);
         } else if (a.nq == 1) {
-            e = launch(cached_attention_kernel<h(), b(), 1, false>, a.wgs, threads, p, 0, s);
+            e = launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, false>, a.wgs, threads, p, 0, s);
         } else {
-            e = launch(cached_attention_kernel<h(), b(), 2, false>, a.wgs, threads, p, 0, s);
+            e = launch(cached_attention_kernel<h(), b(), 2, kAttendWaves, false>, a.wgs, threads, p, 0, s);
         }
         if (e != hipSuccess || a.splits == 1) return e;
         return launch(cached_attention_join_kernel<h(), b()>, ceil_div(rows, 4), 256, p, 0, s);
