@@ -266,6 +266,7 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     p.by_parts = fa::divisor(a.wgs / a.tiles);
     p.by_splits = fa::divisor(a.splits);
     p.by_heads = fa::divisor(cache->heads);
+    p.by_group = fa::divisor(p.group);
     p.scale_log2e = scale * 1.4426950408889634f;
     const int64_t rows = B * L * R;
     p.part_o = static_cast<float*>(workspace);
