@@ -120,42 +120,92 @@ struct AttendPlan {
 
 constexpr int64_t kMostSplits = 64;    // the join gives each a lane
 
-// In how many parts the keys of `base` row tiles are cut.  Microseconds, as measured on 14 shapes (up to 64 sequences, 256 to
-// 131072 tokens; every count of parts; the best one is chosen or one within 5 % of it): a wave takes 1 + H / 110 for a step of 64 tokens, or
-// what the bytes of all waves take at 4.8 TB/s where that is more, workgroups beyond one per compute unit in whole rounds;
-// and the second kernel 3.  (B16 Rkv12 H64, 1000 tokens: 9.9 us in one part, 12.8 in two; Rkv8 H128, 2000 tokens: 18.5 in
-// one part, 12.4 in four, 11.4 in eight; 131072 tokens: 75.7 in 16, 58.5 in 32, 66.1 in 48, 60.7 in 64.)
-int64_t pick_splits(int64_t base, int64_t steps, int64_t H) {
+// A launch and what it takes, in microseconds as measured: `wgs` workgroups of the narrow or the wide kernel for a causal call
+// (what the caller asks for is not known where the workspace is sized, and the longest rows take the same).
+struct Estimate {
+    int64_t splits;
+    float us;
+};
+
+// The second kernel, beside its launch: every split's sums written and read.
+float join_us(const View& p, int64_t splits, int64_t H) {
+    return splits > 1 ? 3.f + (float)p.B * (float)p.L * (float)p.R * (float)splits * (float)H * 8.f / 2.5e6f : 0.f;
+}
+
+// In how many parts the keys of `base` row tiles are cut, few rows.  On 14 shapes (up to 64 sequences, 256 to 131072 tokens)
+// against every other count of parts, the best one is chosen or one within 5 % of it: a wave takes 1 + H / 110 for a step of
+// 64 tokens, or what the bytes of all heads take at 4.8 TB/s where that is more, or the products of a compute unit's
+// workgroups, those beyond one per compute unit in whole rounds; and the second kernel 3.  (B16 Rkv12 H64, 1000 tokens: 9.9 us in one part, 12.8 in two; Rkv8 H128, 2000
+// tokens: 18.5 in one part, 12.4 in four, 11.4 in eight; 131072 tokens: 75.7 in 16, 58.5 in 32, 66.1 in 48, 60.7 in 64.)
+Estimate narrow_splits(const View& p, int64_t base, int64_t steps, int64_t H) {
     const float alone = 1.f + 0.009f * (float)H;
     const float bytes = 0.0273f * (float)H;              // a step of a workgroup's waves, by a 256th of the memory
-    int64_t best = 1;
-    float least = 3.0e38f;
+    const float products = H > 64 ? 1.4f : 0.8f;
+    const int64_t heads = (int64_t)p.B * p.Rkv;
+    Estimate best{1, 3.0e38f};
     for (int64_t s = 1; s <= kMostSplits && (s == 1 || (base * s <= 4 * kNumCu && (s - 1) * fa::cache::kAttendWaves < steps)); ++s) {
-        const int64_t wgs = base * s;
-        const float share = wgs <= kNumCu ? (float)wgs / kNumCu : (float)ceil_div(wgs, kNumCu);
-        const float step = bytes * share > alone ? bytes * share : alone;
-        const float us = step * (float)ceil_div(steps, s * fa::cache::kAttendWaves) + (s > 1 ? 3.f : 0.f);
-        if (us < least) {
-            least = us;
-            best = s;
-        }
+        auto rounds = [](int64_t wgs) { return wgs <= kNumCu ? (float)wgs / kNumCu : (float)ceil_div(wgs, kNumCu); };
+        float step = bytes * rounds(heads * s);
+        if (step < products * rounds(base * s)) step = products * rounds(base * s);
+        if (step < alone) step = alone;
+        const float us = step * (float)ceil_div(steps, s * fa::cache::kAttendWaves) + join_us(p, s, H);
+        if (us < best.us) best = {s, us};
+    }
+    return best;
+}
+
+// Many rows, the narrow kernel in one part: rounds of the workgroups that a chip holds, and what the products and exponentials
+// take in all; or the longest workgroup.  (fp16, causal, estimated and measured: 8 sequences of 1000 tokens of 12 heads of 64: 46, 51 us; 2000 rows
+// of each of 8 heads of 128 over 8000 tokens: 94, 99; 4096 tokens of 32 heads of 128: 251, 247.)
+float narrow_us(const View& p, int64_t base, float keys, int64_t steps, int64_t H) {
+    const int64_t resident = H > 64 ? 2 * kNumCu : 3 * kNumCu;
+    const float rate = H > 64 ? 1.5e6f : H > 32 ? 2.4e6f : 3.e6f;       // rows times keys
+    const float whole = (H > 64 ? 9.f : 6.5f) * (float)ceil_div(base, resident) + (float)p.B * (float)p.L * (float)p.R * keys / rate;
+    const float longest = 6.f + (1.f + 0.009f * (float)H) * (float)ceil_div(steps, fa::cache::kAttendWaves);
+    return whole > longest ? whole : longest;
+}
+
+// The wide kernel: the longest workgroup's tiles of 64 keys, or what the chip's workgroups take in all, of which a compute
+// unit holds one at head_dim 128 and two below.  (The same three: 43, 40 us; 98, 98 in four parts; 145, 172.)
+Estimate wide_us(const View& p, int64_t base, int64_t most_keys, float keys, int64_t H) {
+    Estimate best{1, 3.0e38f};
+    for (int64_t s = 1; s <= kMostSplits && (s == 1 || (base * s <= 4 * kNumCu && s * fa::cache::kWideKeys < most_keys)); ++s) {
+        const float per_cu = (float)(base * s) / kNumCu;
+        const float tile = H > 64 ? 2.17f : (per_cu > 1.f ? 2.3f : 1.6f) - (H > 32 ? 0.f : 0.3f);
+        const float all = H > 64 ? 2.17f * (float)ceil_div(base * s, kNumCu) : 1.15f * per_cu;
+        const float longest = tile * (float)ceil_div(most_keys, s * fa::cache::kWideKeys), whole = all * keys / (float)(s * fa::cache::kWideKeys);
+        const float us = 6.f + (longest > whole ? longest : whole) + join_us(p, s, H);
+        if (us < best.us) best = {s, us};
     }
     return best;
 }
 
 AttendPlan plan_attend(const View& p, int64_t count, int64_t H) {
     AttendPlan a;
-    const int64_t rows = (int64_t)p.L * p.group;
-    a.wide = count == 0 && rows > 64;
+    const int64_t rows = (int64_t)p.L * p.group, heads = (int64_t)p.B * p.Rkv;
+    const int64_t most_keys = (count > 0 ? count : (int64_t)p.W) << p.log2_p, steps = ceil_div(most_keys, 64);
+    a.wide = false;
     a.nq = count > 0 || rows <= 16 ? 1 : 2;
-    a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, a.wide ? fa::cache::kWideRows : 16 * a.nq);
-    const int64_t base = (int64_t)p.B * p.Rkv * a.tiles;
-    a.waves = count > 0 && base > 1000 ? 1 : fa::cache::kAttendWaves;
-    const int64_t steps = ceil_div((count > 0 ? count : (int64_t)p.W) << p.log2_p, 64);     // of 64 tokens
-    a.splits = a.wide ? (base < kNumCu ? kNumCu / base : 1) : a.waves == 1 ? 1 : pick_splits(base, steps, H);
-    if (a.splits > kMostSplits) a.splits = kMostSplits;
-    if (a.splits > steps) a.splits = steps;
-    a.wgs = base * a.splits;
+    a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, 16 * a.nq);
+    a.waves = fa::cache::kAttendWaves;
+    a.splits = 1;
+    const Estimate parts = narrow_splits(p, heads * a.tiles, steps, H);
+    if (count > 0 && heads * a.tiles > 4 * kNumCu)
+        a.waves = 1;                                     // a wave a tile: @@
+    else
+        a.splits = parts.splits;
+    if (count == 0 && rows > 32) {
+        const float keys = most_keys > p.L ? (float)most_keys - 0.5f * (float)p.L : 0.5f * (float)most_keys;
+        const int64_t tiles = ceil_div(rows, fa::cache::kWideRows);
+        const Estimate wide = wide_us(p, heads * tiles, most_keys, keys, H);
+        const float narrow = a.splits > 1 ? parts.us + 6.f : narrow_us(p, heads * a.tiles, keys, steps, H);
+        if (wide.us < narrow) {
+            a.wide = true;
+            a.tiles = tiles;
+            a.splits = wide.splits;
+        }
+    }
+    a.wgs = heads * a.tiles * a.splits;
     return a;
 }
 
@@ -165,7 +215,8 @@ int64_t attend_workspace(const View& p, const AttendPlan& a, int64_t H) {
 
 int check_count(int64_t count) { return count > fa::cache::kMostSelected ? FA_ERR_TOO_LARGE : FA_OK; }
 
-constexpr int kMostTable = 32768;
+constexpr int kMostTable = 32768;        // pages of a table, for a selection: their scores are held in LDS
+constexpr int kMostRowKeys = 8192;       // ... of several tokens: 32 KiB, four workgroups to a compute unit
 
 }  // namespace
 
@@ -322,16 +373,23 @@ int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, in
     (void)workspace;
     (void)workspace_bytes;
     p.by_heads = fa::divisor(p.Rkv);
-    p.by_tokens = fa::divisor(L);
-    const int64_t wgs = (int64_t)p.B * L * p.Rkv;
+    // Several tokens to a workgroup where they share a tile of the product (see the kernel) and there are enough of them to fill
+    // the chip all the same.
+    const int64_t at_once = p.group == 1 || p.group == 2 || p.group == 4 || p.group == 8 ? 16 / p.group : 1;
+    p.tiles = (int)ceil_div(L, at_once);
+    const bool rows = at_once > 1 && at_once * p.W <= kMostRowKeys && (int64_t)p.B * p.tiles * p.Rkv >= kNumCu;
+    const int64_t wgs = (int64_t)p.B * (rows ? p.tiles : L) * p.Rkv;
+    p.by_tokens = fa::divisor(rows ? p.tiles : L);
     if (wgs > kMostThreads / 1024) return FA_ERR_TOO_LARGE;
     const bool many = wgs > 4 * kNumCu;
     return static_cast<int>(for_type(cache->head_dim, (flags & FA_FLAG_BF16) != 0, [&](auto h, auto b) {
         using namespace fa::cache;
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        if (rows) return launch(select_pages_rows_kernel<h(), b()>, wgs, 256, p, (int)at_once * p.W * 4, s);
         auto kernel = many ? select_pages_kernel<h(), b(), 256> : select_pages_kernel<h(), b(), 1024>;
         const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), kMostTable * 4);
         if (e != hipSuccess) return e;
-        return launch(kernel, wgs, many ? 256 : 1024, p, p.W * 4, static_cast<hipStream_t>(stream));
+        return launch(kernel, wgs, many ? 256 : 1024, p, p.W * 4, s);
     }));
 }
 
