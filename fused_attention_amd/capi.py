@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_PKG_DIR, "libfused_attn_gfx950.so")
 # every symbol include/fused_attn.h declares
 EXPORTS = ("fa_fwd", "fa_fwd_ex", "fa_fwd_strided", "fa_fwd_plan", "fa_fwd_variant", "fa_fwd_query", "fa_fwd_reference_bias", "fa_strerror",
            "fa_fwd_timed", "fa_fwd_timed_ex", "fa_qkv_proj", "fa_qkv_proj_plan", "fa_qkv_proj_variant",
-           "fa_cache_append", "fa_cached_attention", "fa_cached_attention_workspace", "fa_select_pages", "fa_select_pages_workspace")
+           "fa_cache_append", "fa_cached_attention", "fa_cached_attention_workspace", "fa_cached_attention_plan", "fa_select_pages", "fa_select_pages_plan")
 FLAG_CAUSAL = 1
 FLAG_BF16 = 2
 
@@ -83,10 +83,12 @@ def load_library():
     lib.fa_cached_attention.restype = ctypes.c_int
     lib.fa_cached_attention_workspace.argtypes = [cache, i64, i64, i64]
     lib.fa_cached_attention_workspace.restype = i64
-    lib.fa_select_pages.argtypes = [cache, vp, i64, i64, i64, vp, i64, vp, vp, i64, i64, ctypes.c_int, vp, i64, vp]
+    lib.fa_cached_attention_plan.argtypes = [cache, i64, i64, i64, ctypes.POINTER(ctypes.c_int)]
+    lib.fa_cached_attention_plan.restype = ctypes.c_int
+    lib.fa_select_pages.argtypes = [cache, vp, i64, i64, i64, vp, i64, vp, vp, i64, i64, ctypes.c_int, vp]
     lib.fa_select_pages.restype = ctypes.c_int
-    lib.fa_select_pages_workspace.argtypes = [cache, i64, i64]
-    lib.fa_select_pages_workspace.restype = i64
+    lib.fa_select_pages_plan.argtypes = [cache, i64, i64, ctypes.POINTER(ctypes.c_int)]
+    lib.fa_select_pages_plan.restype = ctypes.c_int
     lib.fa_strerror.argtypes = [ctypes.c_int]
     lib.fa_strerror.restype = ctypes.c_char_p
     _lib = lib
@@ -524,13 +526,30 @@ def select_pages(queries, key_bounds, k_exponents, page_table, starts, page_size
     if int(count) != count or count < 1:
         raise ValueError("count must be a positive integer, got %r" % (count,))
     _on_one_gpu(tensors + [queries])
-    lib = load_library()
-    nbytes = _bytes(lib.fa_select_pages_workspace(ctypes.byref(c), L, R))
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=queries.device) if nbytes else None
     selected = torch.empty((c.sequences, L, c.heads, count), dtype=torch.int32, device=queries.device)
     with torch.cuda.device(queries.device):
-        _check(lib.fa_select_pages(
+        _check(load_library().fa_select_pages(
             ctypes.byref(c), queries.data_ptr(), *q, selected.data_ptr(), count, starts.data_ptr(),
             new_lens.data_ptr() if new_lens is not None else None, L, R, FLAG_BF16 if queries.dtype == torch.bfloat16 else 0,
-            workspace.data_ptr() if nbytes else None, nbytes, _current_stream(queries) or None))
+            _current_stream(queries) or None))
     return selected
+
+
+def _sizes(B, Rkv, H, P, W, pages=1):
+    return ctypes.byref(Cache(pages=pages, heads=Rkv, page_size=P, head_dim=H, sequences=B, table_width=W, table_stride=W))
+
+
+def cached_attention_plan(B, L, R, Rkv, H, P, W, count=0):
+    """What fa_cached_attention_plan reports for a problem, as a dict.  Needs no GPU."""
+    out = (ctypes.c_int * 5)()
+    _check(load_library().fa_cached_attention_plan(_sizes(B, Rkv, H, P, W), L, R, count, out))
+    res = dict(zip(("kernel", "waves", "rows", "splits", "workgroups"), out))
+    res["kernel"] = ("few", "many")[res["kernel"]]
+    return res
+
+
+def select_pages_plan(B, L, R, Rkv, H, P, W):
+    """What fa_select_pages_plan reports for a problem, as a dict.  Needs no GPU."""
+    out = (ctypes.c_int * 3)()
+    _check(load_library().fa_select_pages_plan(_sizes(B, Rkv, H, P, W), L, R, out))
+    return dict(zip(("tokens", "waves", "workgroups"), out))

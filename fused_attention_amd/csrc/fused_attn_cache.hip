@@ -194,6 +194,7 @@ AttendPlan plan_attend(const View& p, int64_t count, int64_t H) {
         a.waves = 1;                                     // a wave a tile: @@
     else
         a.splits = parts.splits;
+    if (count > 0 && heads * a.tiles <= kNumCu && a.splits <= 2) a.waves = 8, a.splits = 1;
     if (count == 0 && rows > 32) {
         const float keys = most_keys > p.L ? (float)most_keys - 0.5f * (float)p.L : 0.5f * (float)most_keys;
         const int64_t tiles = ceil_div(rows, fa::cache::kWideRows);
@@ -201,6 +202,7 @@ AttendPlan plan_attend(const View& p, int64_t count, int64_t H) {
         const float narrow = a.splits > 1 ? parts.us + 6.f : narrow_us(p, heads * a.tiles, keys, steps, H);
         if (wide.us < narrow) {
             a.wide = true;
+            a.waves = fa::cache::kWideWaves;
             a.tiles = tiles;
             a.splits = wide.splits;
         }
@@ -217,6 +219,26 @@ int check_count(int64_t count) { return count > fa::cache::kMostSelected ? FA_ER
 
 constexpr int kMostTable = 32768;        // pages of a table, for a selection: their scores are held in LDS
 constexpr int kMostRowKeys = 8192;       // ... of several tokens: 32 KiB, four workgroups to a compute unit
+
+// How select_pages is launched: tokens and waves of a workgroup.
+struct SelectPlan {
+    int64_t tokens;
+    int waves;
+    int64_t wgs;
+};
+
+// Several tokens to a workgroup where they share a tile of the product (see the kernel) and there are enough of them to fill the
+// chip all the same (500 tokens of 8 key heads, 250 pages: 18.6 us against 46); otherwise one, with sixteen waves, four where
+// there are more than the chip holds (16 tokens of 8 key heads, 512 pages: 11.9 us against 20 with four).
+SelectPlan plan_select(const View& p) {
+    SelectPlan a;
+    const int64_t heads = (int64_t)p.B * p.Rkv;
+    a.tokens = p.group == 1 || p.group == 2 || p.group == 4 || p.group == 8 ? 16 / p.group : 1;
+    if (a.tokens * p.W > kMostRowKeys || heads * ceil_div(p.L, a.tokens) < kNumCu) a.tokens = 1;
+    a.wgs = heads * ceil_div(p.L, a.tokens);
+    a.waves = a.tokens > 1 || a.wgs > 4 * kNumCu ? 4 : 16;
+    return a;
+}
 
 }  // namespace
 
@@ -333,7 +355,7 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
             e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
             if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
         } else if (count > 0) {
-            e = a.waves == 1 ? launch(cached_attention_kernel<h(), b(), 1, 1, true>, a.wgs, 64, p, list, s)
+            e = a.waves == 8 ? launch(cached_attention_kernel<h(), b(), 1, 8, true>, a.wgs, 512, p, list, s) : a.waves == 1 ? launch(cached_attention_kernel<h(), b(), 1, 1, true>, a.wgs, 64, p, list, s)
                              : launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, true>, a.wgs, threads, p, list, s);
         } else if (a.nq == 1) {
             e = launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, false>, a.wgs, threads, p, 0, s);
@@ -345,17 +367,39 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     }));
 }
 
-int64_t fa_select_pages_workspace(const fa_cache* cache, int64_t L, int64_t R) {
+int fa_cached_attention_plan(const fa_cache* cache, int64_t L, int64_t R, int64_t count, int* plan) {
     View p;
+    if (plan == nullptr) return FA_ERR_NULL_POINTER;
+    int rc = check_sizes(cache, L, R, &p);
+    if (rc == FA_OK) rc = check_count(count);
+    if (rc == FA_OK && count < 0) rc = FA_ERR_BAD_SHAPE;
+    if (rc != FA_OK) return rc;
+    const AttendPlan a = plan_attend(p, count, cache->head_dim);
+    if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
+    plan[0] = a.wide;
+    plan[1] = a.waves;
+    plan[2] = a.wide ? fa::cache::kWideRows : 16 * a.nq;
+    plan[3] = (int)a.splits;
+    plan[4] = (int)a.wgs;
+    return FA_OK;
+}
+
+int fa_select_pages_plan(const fa_cache* cache, int64_t L, int64_t R, int* plan) {
+    View p;
+    if (plan == nullptr) return FA_ERR_NULL_POINTER;
     const int rc = check_sizes(cache, L, R, &p);
     if (rc != FA_OK) return rc;
     if (p.W > kMostTable) return FA_ERR_TOO_LARGE;
-    return 0;
+    const SelectPlan a = plan_select(p);
+    if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
+    plan[0] = (int)a.tokens;
+    plan[1] = a.waves;
+    plan[2] = (int)a.wgs;
+    return FA_OK;
 }
 
 int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, int32_t* selected,
-                    int64_t count, const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R, int flags, void* workspace,
-                    int64_t workspace_bytes, void* stream) {
+                    int64_t count, const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R, int flags, void* stream) {
     if ((flags & ~FA_FLAG_BF16) != 0) return FA_ERR_BAD_FLAGS;
     SelectParams p;
     int rc = check_sizes(cache, L, R, &p);
@@ -370,26 +414,19 @@ int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, in
     p.q = static_cast<const uint16_t*>(q);
     p.selected = selected;
     p.count = (int)count;
-    (void)workspace;
-    (void)workspace_bytes;
+    const SelectPlan a = plan_select(p);
+    if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * a.waves)) return FA_ERR_TOO_LARGE;
     p.by_heads = fa::divisor(p.Rkv);
-    // Several tokens to a workgroup where they share a tile of the product (see the kernel) and there are enough of them to fill
-    // the chip all the same.
-    const int64_t at_once = p.group == 1 || p.group == 2 || p.group == 4 || p.group == 8 ? 16 / p.group : 1;
-    p.tiles = (int)ceil_div(L, at_once);
-    const bool rows = at_once > 1 && at_once * p.W <= kMostRowKeys && (int64_t)p.B * p.tiles * p.Rkv >= kNumCu;
-    const int64_t wgs = (int64_t)p.B * (rows ? p.tiles : L) * p.Rkv;
-    p.by_tokens = fa::divisor(rows ? p.tiles : L);
-    if (wgs > kMostThreads / 1024) return FA_ERR_TOO_LARGE;
-    const bool many = wgs > 4 * kNumCu;
+    p.tiles = (int)ceil_div(L, a.tokens);
+    p.by_tokens = fa::divisor(p.tiles);
     return static_cast<int>(for_type(cache->head_dim, (flags & FA_FLAG_BF16) != 0, [&](auto h, auto b) {
         using namespace fa::cache;
         hipStream_t s = static_cast<hipStream_t>(stream);
-        if (rows) return launch(select_pages_rows_kernel<h(), b()>, wgs, 256, p, (int)at_once * p.W * 4, s);
-        auto kernel = many ? select_pages_kernel<h(), b(), 256> : select_pages_kernel<h(), b(), 1024>;
+        if (a.tokens > 1) return launch(select_pages_rows_kernel<h(), b()>, a.wgs, 64 * a.waves, p, (int)a.tokens * p.W * 4, s);
+        auto kernel = a.waves == 4 ? select_pages_kernel<h(), b(), 256> : select_pages_kernel<h(), b(), 1024>;
         const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), kMostTable * 4);
         if (e != hipSuccess) return e;
-        return launch(kernel, wgs, many ? 256 : 1024, p, p.W * 4, s);
+        return launch(kernel, a.wgs, 64 * a.waves, p, p.W * 4, s);
     }));
 }
 

@@ -637,7 +637,7 @@ const char* fa_strerror(int status) {
         case FA_ERR_BAD_FLAGS: return "fa_fwd_ex: unknown flag, or FA_FLAG_CAUSAL together with a mask";
         case FA_ERR_BAD_SCALE: return "fa_fwd: scale must be finite and positive";
         case FA_ERR_BAD_PAGE: return "fa_cache: page_size must be 16, 32, 64 or 128";
-        case FA_ERR_WORKSPACE: return "fa_cached_attention, fa_select_pages: the workspace is smaller than their _workspace functions say";
+        case FA_ERR_WORKSPACE: return "fa_cached_attention: the workspace is smaller than fa_cached_attention_workspace says";
         default: break;
     }
     if (status > 0) return hipGetErrorString(static_cast<hipError_t>(status));

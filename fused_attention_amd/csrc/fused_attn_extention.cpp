@@ -305,8 +305,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "Appends keys (rotated by their positions) and values to a paged 8-bit cache, in place.  Returns the rotated queries, "
           "or None without queries.");
     m.def("cached_attention",
-          [](torch::Tensor queries, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_exponents, torch::Tensor v_exponents,
-             torch::Tensor page_table, torch::Tensor starts, std::optional<torch::Tensor> new_lens, std::optional<torch::Tensor> pages,
+          [](const torch::Tensor& queries, const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& k_exponents, const torch::Tensor& v_exponents,
+             const torch::Tensor& page_table, const torch::Tensor& starts, const std::optional<torch::Tensor>& new_lens, const std::optional<torch::Tensor>& pages,
              bool causal, bool return_lse, const std::string& layout, std::optional<double> scale) -> py::object {
               const std::vector<torch::Tensor> r = cached_attention(queries, k_cache, v_cache, k_exponents, v_exponents, page_table,
                                                                     starts, new_lens, pages, causal, return_lse, layout, scale);

@@ -301,15 +301,22 @@ int64_t fa_cached_attention_workspace(const fa_cache* cache, int64_t L, int64_t 
  * where q8 = round(q * 2^-e) with the smallest e that keeps the group's queries within 127 (not finite: 0), and largest and
  * smallest are the cache's key_bounds: an upper bound, up to the rounding of q, of what a key of the page can score.  Whole
  * numbers throughout; equal scores go to the lowest place.  Tokens that do not exist get -1 only.
- * q as above, rotated already.  cache->keys, values and value_exponents are not looked at.  table_width is at most 32768
- * (FA_ERR_TOO_LARGE).  workspace as above, fa_select_pages_workspace bytes.
+ * q as above, rotated already.  cache->keys, values and value_exponents are not looked at.  table_width is at most 32768 and
+ * count at most 4096 (FA_ERR_TOO_LARGE).  Needs no workspace.
  */
 int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,
                     int32_t* selected, int64_t count, const int32_t* starts, const int32_t* new_lens,
-                    int64_t L, int64_t R, int flags, void* workspace, int64_t workspace_bytes, void* stream);
+                    int64_t L, int64_t R, int flags, void* stream);
 
-/* Bytes of workspace that fa_select_pages needs, or a negative status, as above. */
-int64_t fa_select_pages_workspace(const fa_cache* cache, int64_t L, int64_t R);
+/*
+ * The launches that fa_cached_attention and fa_select_pages would make for these sizes, without making them (no GPU is touched; only
+ * the sizes in `cache` are looked at): for tests of the launcher and for tuning.  fa_cached_attention_plan fills
+ * plan[0..4] with: 0 = the kernel for few rows, 1 = the one for many; waves per workgroup; query rows per workgroup; parts
+ * that a row's keys are cut into; workgroups.  fa_select_pages_plan fills plan[0..2] with: tokens per workgroup; waves per
+ * workgroup; workgroups.
+ */
+int fa_cached_attention_plan(const fa_cache* cache, int64_t L, int64_t R, int64_t count, int* plan);
+int fa_select_pages_plan(const fa_cache* cache, int64_t L, int64_t R, int* plan);
 
 #ifdef __cplusplus
 }

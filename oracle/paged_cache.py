@@ -148,21 +148,26 @@ def attention(cache, q, starts, lens, selected=None, causal=True, scale=None):
             if not keys:
                 continue
             keys, values, at = np.concatenate(keys), np.concatenate(values), np.concatenate(at)
-            for i in range(L):
-                seen = at < _visible(cache, starts, lens, b, i, L, causal)
-                if selected is not None:
-                    seen &= np.isin(at // cache.P, selected[b, i, head].numpy())
-                if not seen.any():
-                    continue
-                for r in range(head * group, (head + 1) * group):
-                    with np.errstate(invalid="ignore"):
-                        s = keys[seen] @ x[b, i, r] * scale
-                        top = s.max()
-                        p = np.exp(s - top)
-                        out[b, i, r] = p @ values[seen] / p.sum()
-                        spread[b, i, r] = p @ np.abs(values[seen]) / p.sum()
-                        lse[b, r, i] = top + np.log(p.sum())
-                        size[b, i, r] = (np.abs(keys[seen]) @ np.abs(x[b, i, r])).max() * scale
+            rows = slice(head * group, (head + 1) * group)
+            seen = at < np.array([_visible(cache, starts, lens, b, i, L, causal) for i in range(L)])[:, None]      # [L, keys]
+            if selected is not None:
+                seen &= np.stack([np.isin(at // cache.P, selected[b, i, head].numpy()) for i in range(L)])
+            seen = np.repeat(seen, group, axis=0)                  # a row per token and query head
+            with np.errstate(invalid="ignore", divide="ignore"):
+                y = x[b, :, rows].reshape(L * group, H)
+                s = np.where(seen, y @ keys.T * scale, -np.inf)
+                top = s.max(axis=1, keepdims=True)
+                p = np.where(seen, np.exp(s - np.where(top == -np.inf, 0.0, top)), 0.0)
+                total = p.sum(axis=1, keepdims=True)
+                # a NaN that a row does not see is none of its business: zero in its place, and counted apart
+                bad = np.isnan(values)
+                o = p @ np.where(bad, 0.0, values) / np.where(total == 0, 1.0, total)
+                o[(seen.astype(np.float64) @ bad) > 0] = np.nan
+                a = p @ np.where(bad, 0.0, np.abs(values)) / np.where(total == 0, 1.0, total)
+                z = np.where(seen, np.abs(y) @ np.abs(keys).T, 0.0).max(axis=1) * scale
+                out[b, :, rows], spread[b, :, rows] = o.reshape(L, group, H), a.reshape(L, group, H)
+                lse[b, rows] = np.where(total == 0, -np.inf, top + np.log(total))[:, 0].reshape(L, group).T
+                size[b, :, rows] = z.reshape(L, group)
     return torch.from_numpy(out), torch.from_numpy(lse), torch.from_numpy(spread), torch.from_numpy(size)
 
 

@@ -220,7 +220,7 @@ def test_the_library_refuses_what_its_header_says():
                                        None)
 
     def select(c=None, q=ok, qs=(512, 64, 256), sel=ok, count=2, starts=ok, lens=None, L=2, R=4, flags=0):
-        return lib.fa_select_pages(cache() if c is None else c, q, *qs, sel, count, starts, lens, L, R, flags, None, 0, None)
+        return lib.fa_select_pages(cache() if c is None else c, q, *qs, sel, count, starts, lens, L, R, flags, None)
 
     for call in (append, attend, select):
         assert call(c=cache(head_dim=48)) == -2 and call(c=cache(head_dim=256)) == -2
@@ -261,7 +261,11 @@ def test_the_library_refuses_what_its_header_says():
     assert attend(c=cache(**long), L=1) == -10 and attend(c=cache(**long), L=1, ws=ok, n=need - 1) == -10
     assert attend(c=cache(**long), L=1, ws=ok + 4, n=need) == -5
     assert lib.fa_cached_attention_workspace(cache(head_dim=3), 1, 4, 0) == -2 and lib.fa_cached_attention_workspace(cache(), 1, 4, 5000) == -6
-    assert lib.fa_select_pages_workspace(cache(page_size=3), 1, 4) == -9
+    plan = (ctypes.c_int * 5)()
+    assert lib.fa_cached_attention_plan(cache(), 1, 4, 0, None) == -1 and lib.fa_select_pages_plan(cache(), 1, 4, None) == -1
+    assert lib.fa_cached_attention_plan(cache(page_size=3), 1, 4, 0, plan) == -9 and lib.fa_cached_attention_plan(cache(), 1, 4, -1, plan) == -3
+    assert lib.fa_cached_attention_plan(cache(), 1, 4, 5000, plan) == -6 and lib.fa_select_pages_plan(cache(heads=3), 1, 4, plan) == -3
+    assert lib.fa_select_pages_plan(cache(table_width=32769, table_stride=32769, page_size=16), 1, 4, plan) == -6
     assert "page_size" in capi.strerror(-9) and "workspace" in capi.strerror(-10)
 
 
@@ -515,9 +519,62 @@ def test_append_writes_nothing_else(gpu):
 ])
 @pytest.mark.parametrize("causal", [True, False])
 def test_attention_is_the_oracles(gpu, dtype, H, P, R, Rkv, L, W, layout, causal):
-    p = Problem(B=3, L=L, R=R, Rkv=Rkv, H=H, P=P, W=W, dtype=dtype, seed=H + P + L, layout=layout)
-    p.starts = [W * P - L, max(0, (W * P - L) // 2 - 3), 0]
-    p.lens = [L, L - L // 4, L]
+    _compare_attention(gpu, 3, dtype, H, P, R, Rkv, L, W, layout, causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,H,P,R,Rkv,L,W,layout", [
+    (32, 16, 16, 24, 8, 40, 4, "blf"),
+    (1, 16, 32, 12, 4, 500, 100, "blf"),   # keys in parts
+    (48, 32, 16, 16, 2, 40, 4, "bhld"),
+    (8, 32, 64, 6, 2, 130, 100, "blf"),    # keys in parts, head_dim 32
+    (16, 64, 64, 16, 8, 100, 2, "blf"),
+    (32, 64, 16, 8, 8, 100, 8, "bhld"),
+    (1, 128, 16, 8, 1, 40, 4, "blf"),      # two tiles of rows
+    (1, 128, 32, 3, 1, 45, 2, "blf"),      # three query heads to a key head, rows that end inside a wave's
+    (4, 128, 64, 64, 8, 70, 2, "bhld"),
+    (1, 128, 64, 64, 8, 130, 100, "blf"),  # keys in parts, head_dim 128
+])
+def test_attention_of_many_rows_is_the_oracles(gpu, dtype, B, H, P, R, Rkv, L, W, layout):
+    assert capi.cached_attention_plan(B, L, R, Rkv, H, P, W)["kernel"] == "many"
+    for causal in (True, False):
+        _compare_attention(gpu, B, dtype, H, P, R, Rkv, L, W, layout, causal)
+
+
+def test_launches_are_within_what_the_kernels_take():
+    # as the kernels count on: row tiles times parts times heads, lanes for the join, parts with keys to take
+    rng = random.Random(5)
+    kinds = set()
+    for _ in range(4000):
+        H, P = rng.choice([16, 32, 64, 128]), rng.choice([16, 32, 64, 128])
+        B, Rkv, group = int(2 ** rng.uniform(0, 8)), rng.choice([1, 2, 3, 8, 16]), rng.choice([1, 2, 3, 4, 5, 8, 17, 64])
+        L, W = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 12))
+        count = rng.choice([0, 0, 0, rng.randint(1, 4096)])
+        plan = capi.cached_attention_plan(B, L, Rkv * group, Rkv, H, P, W, count)
+        rows = plan["rows"]
+        tiles = L * -(-group // rows) if count else -(-L * group // rows)
+        keys = (count or W) * P
+        assert plan["workgroups"] == B * Rkv * tiles * plan["splits"]
+        assert 1 <= plan["splits"] <= 64 and (plan["splits"] - 1) * 64 < keys
+        if plan["kernel"] == "many":
+            assert (plan["waves"], rows) == (8, 256) and not count
+        else:
+            assert plan["waves"] == 4 or (count and plan["waves"] in (1, 8))
+            assert rows in (16, 32) and (rows == 16 or (L * group > 16 and not count))
+        kinds.add((plan["kernel"], plan["waves"], rows, plan["splits"] > 1))
+        if W <= 2048:
+            plan = capi.select_pages_plan(B, L, Rkv * group, Rkv, H, P, W)
+            assert plan["workgroups"] == B * Rkv * -(-L // plan["tokens"])
+            assert plan["tokens"] == 1 or (plan["tokens"] * group == 16 and plan["tokens"] * W <= 8192 and plan["waves"] == 4)
+            kinds.add(("select", plan["tokens"] > 1, plan["waves"]))
+    assert len(kinds) == 6 + 2 + 3, kinds                         # few rows, many rows, selections
+
+
+def _compare_attention(gpu, B, dtype, H, P, R, Rkv, L, W, layout, causal):
+    p = Problem(B=B, L=L, R=R, Rkv=Rkv, H=H, P=P, W=W, dtype=dtype, seed=H + P + L, layout=layout)
+    p.starts = ([W * P - L, max(0, (W * P - L) // 2 - 3), 0] + [(7 * b) % (W * P - L + 1) for b in range(B)])[:B]
+    p.lens = ([L, L - L // 4, L] + [L - b % L for b in range(B)])[:B]
     want = pc.attention(p.cache(), p.q, p.starts, p.lens, causal=causal)
     for m in (_entries(), capi):
         t = p.on(gpu)
@@ -541,30 +598,35 @@ def test_attention_over_long_tables(gpu, W, P, B, starts):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_attention_over_rows_that_see_nothing(gpu, dtype):
-    p = Problem(B=6, L=20, R=4, Rkv=2, H=64, P=16, W=4, dtype=dtype, seed=7)
+@pytest.mark.parametrize("H,R,L,kernel", [(64, 4, 20, "few"), (128, 32, 64, "many")])
+def test_attention_over_rows_that_see_nothing(gpu, dtype, H, R, L, kernel):
+    p = Problem(B=6, L=L, R=R, Rkv=2, H=H, P=16, W=4, dtype=dtype, seed=7)
+    assert capi.cached_attention_plan(6, L, R, 2, H, 16, 4)["kernel"] == kernel
     N = p.k_cache.shape[0]
     p.page_table[1] = -1                                           # no page at all
     p.page_table[2] = torch.tensor([N, 3, -9, 2 ** 31 - 1])
     p.page_table[5, 0] = -1                                        # the first tokens' page is missing
     p.starts = [44, 44, 30, 100, -7, 0]                            # behind the table; before zero
-    p.lens = [0, 20, 20, 20, 20, 20]
+    p.lens = [0] + [L] * 5
     for causal in (True, False):
         want = pc.attention(p.cache(), p.q, p.starts, p.lens, causal=causal)
         got, lse = _attend(_entries(), p, p.on(gpu), causal=causal, return_lse=True)
-        _check_attention(p, p.by_token(got, 4), lse, want)
-    p.starts, p.lens = [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 5, 40, 0, 63], [20, 20, -3, 500, -2 ** 31, 1]
+        _check_attention(p, p.by_token(got, R), lse, want)
+    p.starts, p.lens = [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 5, 40, 0, 63], [L, L, -3, 500, -2 ** 31, 1]
+    p.q[3, L - 1], p.q[5, 1:] = math.nan, math.inf                 # rows that do not exist hold anything
+    p.lens[3] = L - 1
     want = pc.attention(p.cache(), p.q, p.starts, p.lens)
     got, lse = _attend(_entries(), p, p.on(gpu), return_lse=True)
-    _check_attention(p, p.by_token(got, 4), lse, want)
+    _check_attention(p, p.by_token(got, R), lse, want)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("L,R", [(1, 4), (20, 4), (150, 2)])
+@pytest.mark.parametrize("H,L,R,kernel", [(64, 1, 4, "few"), (64, 20, 4, "few"), (64, 150, 2, "few"), (128, 150, 64, "many")])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_values_that_are_not_numbers_stay_where_they_are_seen(gpu, dtype, L, R):
+def test_values_that_are_not_numbers_stay_where_they_are_seen(gpu, dtype, H, L, R, kernel):
     # behind the last token, on pages that nobody names, and in tokens that some rows of a tile see and others do not
-    p = Problem(B=2, L=L, R=R, Rkv=2, H=64, P=16, W=12, dtype=dtype, seed=8 + L)
+    p = Problem(B=2, L=L, R=R, Rkv=2, H=H, P=16, W=12, dtype=dtype, seed=8 + L)
+    assert capi.cached_attention_plan(2, L, R, 2, H, 16, 12)["kernel"] == kernel
     p.starts = [12 * 16 - L - 30, 5]
     nan = torch.tensor(0x7f, dtype=torch.uint8)
     clean_k, clean_v = p.k_cache.clone(), p.v_cache.clone()
@@ -596,21 +658,23 @@ def test_values_that_are_not_numbers_stay_where_they_are_seen(gpu, dtype, L, R):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_attention_over_pages_of_different_sizes(gpu, dtype):
+@pytest.mark.parametrize("H,R,L,kernel", [(64, 4, 9, "few"), (128, 128, 90, "many")])
+def test_attention_over_pages_of_different_sizes(gpu, dtype, H, R, L, kernel):
     # exponents that grow and shrink along a sequence, scores far apart, scales of the caller's
-    p = Problem(B=2, L=9, R=4, Rkv=2, H=64, P=16, W=10, dtype=dtype, seed=9)
-    p.starts = [150, 77]
+    p = Problem(B=2, L=L, R=R, Rkv=2, H=H, P=16, W=10, dtype=dtype, seed=9)
+    assert capi.cached_attention_plan(2, L, R, 2, H, 16, 10)["kernel"] == kernel
+    p.starts = [160 - L, 70]
     p.k_exponents += torch.randint(-2, 3, p.k_exponents.shape, generator=p.gen).to(torch.int8)
     p.v_exponents += torch.randint(-6, 7, p.v_exponents.shape, generator=p.gen).to(torch.int8)
     for scale in (None, 0.9, 1e-4):
         want = pc.attention(p.cache(), p.q, p.starts, p.lens, scale=scale)
         got, lse = _attend(_entries(), p, p.on(gpu), return_lse=True, scale=scale)
-        _check_attention(p, p.by_token(got, 4), lse, want)
+        _check_attention(p, p.by_token(got, R), lse, want)
     if dtype == torch.bfloat16:                                    # values far outside of fp16
         p.v_exponents += 60
         want = pc.attention(p.cache(), p.q, p.starts, p.lens)
         got = _attend(_entries(), p, p.on(gpu))
-        _check_attention(p, p.by_token(got, 4), None, want)
+        _check_attention(p, p.by_token(got, R), None, want)
 
 
 @pytest.mark.gpu
@@ -618,6 +682,9 @@ def test_attention_over_pages_of_different_sizes(gpu, dtype):
 @pytest.mark.parametrize("H,P,R,Rkv,L,W,count,layout", [
     (64, 16, 2, 2, 1, 1, 1, "blf"), (64, 16, 4, 2, 3, 12, 4, "bhld"), (128, 64, 20, 4, 1, 30, 8, "blf"), (128, 32, 32, 1, 2, 9, 5, "blf"),
     (16, 128, 4, 2, 5, 6, 3, "blf"), (32, 64, 6, 3, 30, 5, 2, "bhld"), (64, 16, 8, 2, 2, 300, 64, "blf"), (128, 16, 40, 1, 1, 600, 33, "blf"),
+    # sixteen rows of several tokens to a workgroup of the selection, and more attention tiles than a chip holds
+    (64, 16, 8, 8, 300, 25, 5, "blf"), (16, 16, 16, 8, 150, 12, 4, "bhld"), (128, 32, 32, 8, 70, 40, 9, "blf"), (32, 64, 64, 8, 35, 5, 3, "blf"),
+    (64, 16, 24, 8, 120, 20, 20, "blf"),
 ])
 def test_selection_and_attention_over_it_are_the_oracles(gpu, dtype, H, P, R, Rkv, L, W, count, layout):
     p = Problem(B=2, L=L, R=R, Rkv=Rkv, H=H, P=P, W=W, dtype=dtype, seed=H + W, layout=layout)
@@ -630,6 +697,8 @@ def test_selection_and_attention_over_it_are_the_oracles(gpu, dtype, H, P, R, Rk
     want = pc.attention(cache, p.q, p.starts, p.lens, selected=want_pages)
     for m in (_entries(), capi):
         t = p.on(gpu)
+        plan = capi.select_pages_plan(2, L, R, Rkv, H, P, W)
+        assert (plan["tokens"] > 1) == (L > 30 and R // Rkv in (1, 2, 4, 8))
         pages = _select(m, p, t, count)
         assert torch.equal(pages.cpu(), want_pages)
         got, lse = _attend(m, p, t, pages=pages, return_lse=True)
@@ -637,10 +706,11 @@ def test_selection_and_attention_over_it_are_the_oracles(gpu, dtype, H, P, R, Rk
 
 
 @pytest.mark.gpu
-def test_selections_with_ties_and_odd_queries(gpu):
+@pytest.mark.parametrize("L,R,Rkv", [(2, 4, 2), (90, 16, 8), (45, 4, 4)])
+def test_selections_with_ties_and_odd_queries(gpu, L, R, Rkv):
     m = _entries()
-    p = Problem(B=3, L=2, R=4, Rkv=2, H=64, P=16, W=40, seed=11)
-    p.starts = [600, 333, 0]
+    p = Problem(B=3, L=L, R=R, Rkv=Rkv, H=64, P=16, W=40, seed=11)
+    p.starts = [640 - L, 333, 0]
     p.key_bounds[:, :, 0], p.key_bounds[:, :, 1] = 1, -1          # every page the same score
     p.k_exponents[:] = -7
     for count in (1, 2, 7, 39, 40, 64):
@@ -654,7 +724,7 @@ def test_selections_with_ties_and_odd_queries(gpu):
     p.key_bounds[:, :, 0], p.key_bounds[:, :, 1] = -3, -90
     p.q = p.q.nan_to_num(posinf=9.0).abs()
     p.k_exponents[:] = torch.randint(-80, 121, p.k_exponents.shape, generator=p.gen).to(torch.int8)
-    p.starts = [638, 400, -9]
+    p.starts, p.lens = [638, 400, -1], [L, L - 1, L]
     assert torch.equal(_select(m, p, p.on(gpu), 9).cpu(), pc.select(p.cache(), p.q, p.starts, p.lens, 9))
 
 
