@@ -279,6 +279,10 @@ int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t
     p.reach = (int)(reach < p.W ? reach : p.W);
     p.cache_items = B * p.reach * cache->heads * 2;
     p.q_units = q != nullptr ? B * L * R * (H / 16) : 0;
+    p.by_query_heads = fa::divisor(p.R);
+    p.by_tokens = fa::divisor(L);
+    p.by_heads = fa::divisor(p.Rkv);
+    p.by_reach = fa::divisor(p.reach);
     const bool bf = (flags & FA_FLAG_BF16) != 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t units = (L < P ? L : P) * (H / 16);    // of a page's new tokens
