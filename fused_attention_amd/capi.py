@@ -523,8 +523,8 @@ def select_pages(queries, key_bounds, k_exponents, page_table, starts, page_size
         raise ValueError("key_bounds must be [pages, key heads, 2, head_dim], got %s" % (tuple(key_bounds.shape),))
     c, tensors = _cache(k_exponents, page_table, starts, new_lens, page_size, key_bounds.shape[3], key_bounds=key_bounds)
     L, R, q = _query_tokens(queries, None, layout, c)
-    if int(count) != count or count < 1:
-        raise ValueError("count must be a positive integer, got %r" % (count,))
+    if int(count) != count or not 1 <= count <= 4096:
+        raise ValueError("count must be between 1 and 4096, got %r" % (count,))
     _on_one_gpu(tensors + [queries])
     selected = torch.empty((c.sequences, L, c.heads, count), dtype=torch.int32, device=queries.device)
     with torch.cuda.device(queries.device):

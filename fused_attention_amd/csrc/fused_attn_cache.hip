@@ -360,6 +360,11 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
             e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
             if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
         } else if (count > 0) {
+            const void* kernel = a.waves == 8   ? reinterpret_cast<const void*>(cached_attention_kernel<h(), b(), 1, 8, true>)
+                                 : a.waves == 1 ? reinterpret_cast<const void*>(cached_attention_kernel<h(), b(), 1, 1, true>)
+                                                : reinterpret_cast<const void*>(cached_attention_kernel<h(), b(), 1, kAttendWaves, true>);
+            e = allow_large_lds(kernel, kMostSelected * 4);      // beside up to 64 KiB of its own
+            if (e != hipSuccess) return e;
             e = a.waves == 8 ? launch(cached_attention_kernel<h(), b(), 1, 8, true>, a.wgs, 512, p, list, s) : a.waves == 1 ? launch(cached_attention_kernel<h(), b(), 1, 1, true>, a.wgs, 64, p, list, s)
                              : launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, true>, a.wgs, threads, p, list, s);
         } else if (a.nq == 1) {

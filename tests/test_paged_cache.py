@@ -360,6 +360,7 @@ def test_the_entry_points_refuse_wrong_tensors(how):
     refused("pages must be", ("attend",), pages=pages[:, :2])
     refused("pages must be", ("attend",), pages=pages[..., :0])
     refused("count must be", ("select",), count=0)
+    refused("count must be", ("select",), count=4097)
 
 
 # ---- on the GPU ----
@@ -744,6 +745,29 @@ def test_lists_of_pages_as_they_come(gpu):
     want = pc.attention(p.cache(), p.q, p.starts, p.lens)
     got, lse = _attend(_entries(), p, p.on(gpu), pages=many.to(gpu), return_lse=True)
     _check_attention(p, p.by_token(got, 4), lse, want)
+
+
+@pytest.mark.gpu
+def test_the_widest_table_and_the_longest_lists(gpu):
+    # 32768 pages in a table, 4096 of them selected; the longest lists on each form of the attention kernel
+    m = _entries()
+    p = Problem(B=1, L=2, R=2, Rkv=1, H=16, P=16, W=32768, seed=20, extra=0)
+    p.starts = [32768 * 16 - 2]
+    pages = _select(m, p, p.on(gpu), 4096)
+    cache = p.cache()
+    want = pc.select(cache, p.q, p.starts, p.lens, 4096)
+    assert torch.equal(pages.cpu(), want)
+    got, lse = _attend(m, p, p.on(gpu), pages=pages, return_lse=True)
+    _check_attention(p, p.by_token(got, 2), lse, pc.attention(cache, p.q, p.starts, p.lens, selected=want))
+    for B, L, waves in ((2, 1, 4), (100, 1, 8), (3, 200, 1)):
+        p = Problem(B=B, L=L, R=2, Rkv=2, H=128, P=16, W=16, seed=21)
+        assert capi.cached_attention_plan(B, L, 2, 2, 128, 16, 16, 4096)["waves"] == waves
+        p.starts = [(31 * b) % (256 - L + 1) for b in range(B)]
+        lists = torch.full((B, L, 2, 4096), -1, dtype=torch.int32)
+        lists[..., 5], lists[..., 100], lists[..., 101], lists[..., 4095] = 3, 9, 3, 0
+        want = pc.attention(p.cache(), p.q, p.starts, p.lens, selected=lists)
+        got, lse = _attend(m, p, p.on(gpu), pages=lists.to(gpu), return_lse=True)
+        _check_attention(p, p.by_token(got, 2), lse, want)
 
 
 @pytest.mark.gpu
