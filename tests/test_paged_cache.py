@@ -748,6 +748,20 @@ def test_lists_of_pages_as_they_come(gpu):
 
 
 @pytest.mark.gpu
+def test_lists_with_gaps(gpu):
+    # a page named on both sides of numbers that name nothing still counts once
+    p = Problem(B=2, L=3, R=4, Rkv=2, H=64, P=16, W=6, seed=22)
+    p.starts = [90, 40]
+    lists = [[5, -1, 5, -1, 5, -1], [0, 1, -1, 0, 1, 2], [-1, 2, -5, 2, 3, 4], [1, 6, -1, 1, 6, -1], [-1, -1, 3, 4, -1, 3], [0, -2 ** 31, 0, 2, 2 ** 31 - 1, 2]]
+    pages = torch.tensor(lists * 2, dtype=torch.int32).view(2, 3, 2, 6)
+    for repeats in (1, 60):                              # entries of one thread, and of several
+        some = torch.cat([pages] * repeats, dim=3)
+        want = pc.attention(p.cache(), p.q, p.starts, p.lens, selected=some)
+        got, lse = _attend(_entries(), p, p.on(gpu), pages=some.to(gpu), return_lse=True)
+        _check_attention(p, p.by_token(got, 4), lse, want)
+
+
+@pytest.mark.gpu
 def test_the_widest_table_and_the_longest_lists(gpu):
     # 32768 pages in a table, 4096 of them selected; the longest lists on each form of the attention kernel
     m = _entries()
