@@ -4,6 +4,7 @@
 
 #include "../../include/fused_attn.h"
 
+#include <cmath>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -346,6 +347,9 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     p.by_heads = fa::divisor(cache->heads);
     p.by_group = fa::divisor(p.group);
     p.scale_log2e = scale * 1.4426950408889634f;
+    int power;                                           // scale_log2e is at least 2^(power - 1)
+    std::frexp(p.scale_log2e, &power);
+    p.least_exponent = -125 - power;
     const int64_t rows = B * L * R;
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + rows * a.splits * H;

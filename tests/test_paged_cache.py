@@ -679,6 +679,23 @@ def test_attention_over_pages_of_different_sizes(gpu, dtype, H, R, L, kernel):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,R,L,kernel", [(64, 4, 9, "few"), (64, 256, 90, "many"), (128, 128, 90, "many")])
+def test_scores_too_small_for_a_factor(gpu, H, R, L, kernel):
+    # the caller's scale times a page's power of two below any float32: what a row does not see stays out of it all the same
+    p = Problem(B=2, L=L, R=R, Rkv=2, H=H, P=16, W=10, seed=23)
+    assert capi.cached_attention_plan(2, L, R, 2, H, 16, 10)["kernel"] == kernel
+    p.starts = [150 - L, 70]
+    pages = torch.randint(0, 10, (2, L, 2, 4), generator=p.gen).to(torch.int32)
+    for exponent, scale in ((None, 1e-30), (-80, 1e-30), (-128, 1e-6), (None, 1e-38)):
+        if exponent is not None:
+            p.k_exponents[::2] = exponent
+        for selected in (None, pages):
+            want = pc.attention(p.cache(), p.q, p.starts, p.lens, scale=scale, selected=selected)
+            got, lse = _attend(_entries(), p, p.on(gpu), return_lse=True, scale=scale, **({} if selected is None else {"pages": selected.to(gpu)}))
+            _check_attention(p, p.by_token(got, R), lse, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("H,P,R,Rkv,L,W,count,layout", [
     (64, 16, 2, 2, 1, 1, 1, "blf"), (64, 16, 4, 2, 3, 12, 4, "bhld"), (128, 64, 20, 4, 1, 30, 8, "blf"), (128, 32, 32, 1, 2, 9, 5, "blf"),
