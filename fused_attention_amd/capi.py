@@ -424,9 +424,13 @@ def _on_one_gpu(tensors):
 
 
 def _query_tokens(queries, out, layout, c):
+    import torch
+
     L, R, strides = _tokens("queries", queries, layout, c)
     if R % c.heads != 0:
         raise ValueError("the heads of queries (%d) must be a multiple of the key heads (%d)" % (R, c.heads))
+    if out is not None and not isinstance(out, torch.Tensor):
+        raise TypeError("out must be a torch.Tensor, got %s" % type(out).__name__)
     if out is not None and (out.shape != queries.shape or out.dtype != queries.dtype):
         raise ValueError("out must have the shape and dtype of queries")
     return L, R, strides
@@ -439,14 +443,14 @@ def cache_append(keys, values, k_cache, v_cache, k_exponents, v_exponents, page_
     given), or None without queries.  The cache's tensors are described in include/fused_attn.h."""
     import torch
 
-    if k_cache.dim() != 4:
+    if _kind("k_cache", k_cache, torch.float8_e4m3fn).dim() != 4:
         raise ValueError("k_cache must be [pages, key heads, page_size, head_dim], got %s" % (tuple(k_cache.shape),))
     c, tensors = _cache(k_exponents, page_table, starts, new_lens, k_cache.shape[2], k_cache.shape[3], k_cache, v_cache, v_exponents,
                         key_bounds)
     L, heads, kv = _tokens("keys", keys, layout, c)
     if heads != c.heads:
         raise ValueError("keys must have the key heads of the cache (%d), got %d" % (c.heads, heads))
-    if values.dtype != keys.dtype or values.shape != keys.shape or _tokens("values", values, layout, c)[2] != kv:
+    if _tokens("values", values, layout, c) != (L, heads, kv) or values.dtype != keys.dtype or values.shape != keys.shape:
         raise ValueError("values must have the dtype, shape and strides of keys")
     R, q, o = c.heads, (0, 0, 0), (0, 0, 0)
     if queries is None and out is not None:
@@ -463,7 +467,9 @@ def cache_append(keys, values, k_cache, v_cache, k_exponents, v_exponents, page_
             raise ValueError("rope must be a pair (cos, sin) of float32 [positions, head_dim / 2] tensors")
         tables = tuple(rope)
         for name, t in zip(("rope cos", "rope sin"), tables):
-            _kind(name, t, torch.float32, (tables[0].shape[0], c.head_dim // 2))
+            _kind(name, t, torch.float32)
+            if tuple(t.shape) != (len(tables[0]), c.head_dim // 2) or len(t) == 0:
+                raise ValueError("%s must be [positions, head_dim / 2 = %d], one shape for both, got %s" % (name, c.head_dim // 2, tuple(t.shape)))
     _on_one_gpu(tensors + [keys, values] + [t for t in (queries, out) + tables if t is not None])
     with torch.cuda.device(keys.device):
         _check(load_library().fa_cache_append(
@@ -488,7 +494,7 @@ def cached_attention(queries, k_cache, v_cache, k_exponents, v_exponents, page_t
     (out, lse)."""
     import torch
 
-    if k_cache.dim() != 4:
+    if _kind("k_cache", k_cache, torch.float8_e4m3fn).dim() != 4:
         raise ValueError("k_cache must be [pages, key heads, page_size, head_dim], got %s" % (tuple(k_cache.shape),))
     c, tensors = _cache(k_exponents, page_table, starts, new_lens, k_cache.shape[2], k_cache.shape[3], k_cache, v_cache, v_exponents)
     L, R, q = _query_tokens(queries, out, layout, c)
@@ -519,7 +525,7 @@ def select_pages(queries, key_bounds, k_exponents, page_table, starts, page_size
     """fa_select_pages on torch GPU tensors, on torch's current stream.  Returns int32 [batch, seq_len, key heads, count]."""
     import torch
 
-    if key_bounds.dim() != 4:
+    if _kind("key_bounds", key_bounds, torch.int8).dim() != 4:
         raise ValueError("key_bounds must be [pages, key heads, 2, head_dim], got %s" % (tuple(key_bounds.shape),))
     c, tensors = _cache(k_exponents, page_table, starts, new_lens, page_size, key_bounds.shape[3], key_bounds=key_bounds)
     L, R, q = _query_tokens(queries, None, layout, c)

@@ -78,6 +78,12 @@ int check_strided(const void* t, const Strides3& s, int64_t B, int64_t heads, in
     return FA_OK;
 }
 
+// What is written: the same, with a place of its own for every row.
+int check_written(const void* t, const Strides3& s, int64_t B, int64_t heads, int64_t L, int64_t H) {
+    if ((s.b == 0 && B > 1) || (s.h == 0 && heads > 1)) return FA_ERR_BAD_STRIDE;
+    return check_strided(t, s, B, heads, L, H);
+}
+
 // Dynamic LDS above 64 KiB has to be opted into per kernel function and per device.
 hipError_t allow_large_lds(const void* kernel, int bytes) {
     static std::mutex lock;
@@ -263,7 +269,7 @@ int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t
         if ((rc = check_strided(t, p.kv, B, cache->heads, L, H)) != FA_OK) return rc;
     if ((q == nullptr) != (q_out == nullptr)) return FA_ERR_NULL_POINTER;
     if (q != nullptr && (rc = check_strided(q, p.qs, B, R, L, H)) != FA_OK) return rc;
-    if (q != nullptr && (rc = check_strided(q_out, p.qo, B, R, L, H)) != FA_OK) return rc;
+    if (q != nullptr && (rc = check_written(q_out, p.qo, B, R, L, H)) != FA_OK) return rc;
     if ((rope_cos == nullptr) != (rope_sin == nullptr)) return FA_ERR_NULL_POINTER;
     if (rope_cos != nullptr && rope_rows < 1) return FA_ERR_BAD_SHAPE;
     if (!aligned(rope_cos, 16) || !aligned(rope_sin, 16)) return FA_ERR_MISALIGNED;
@@ -327,7 +333,7 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     p.qs = {q_stride_b, q_stride_h, q_stride_l};
     p.os = {out_stride_b, out_stride_h, out_stride_l};
     if ((rc = check_strided(q, p.qs, B, R, L, H)) != FA_OK) return rc;
-    if ((rc = check_strided(out, p.os, B, R, L, H)) != FA_OK) return rc;
+    if ((rc = check_written(out, p.os, B, R, L, H)) != FA_OK) return rc;
     if (!aligned(lse, 4) || !aligned(selected, 4)) return FA_ERR_MISALIGNED;
     const AttendPlan a = plan_attend(p, count, H);
     if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * fa::cache::kWideWaves)) return FA_ERR_TOO_LARGE;

@@ -261,6 +261,7 @@ typedef struct fa_cache {
  * A page that a call writes must belong to one sequence and stand once in its table.
  * q (nullable, strides q_stride_*, R heads) is rotated likewise into q_out (strides out_stride_*, not overlapping q),
  * rounded once; rows of tokens that do not exist, or from rope_rows on, become zeros.  R is not looked at without q.
+ * Strides of 0 are for k, v and q only (FA_ERR_BAD_STRIDE for q_out, here, and out, below).
  */
 int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t kv_stride_b, int64_t kv_stride_h, int64_t kv_stride_l,
                     const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,

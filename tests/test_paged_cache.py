@@ -246,6 +246,7 @@ def test_the_library_refuses_what_its_header_says():
             assert call(c=cache(**{name: None})) == -1, name
         assert call(c=cache(keys=ok + 8)) == -5 and call(c=cache(values=ok + 4)) == -5
         assert call(out=None) == -1 and call(os=(512, 64, 8)) == -4 and call(out=ok + 8) == -5
+        assert call(os=(0, 64, 256)) == -4 and call(os=(512, 0, 256)) == -4        # rows in one place
     assert append(k=None) == -1 and append(v=ok + 8) == -5 and append(kv=(512, 64, 60)) == -4
     assert append(q=None, out=ok) == -1
     assert append(cos=ok) == -1 and append(cos=ok, sin=ok, rows=0) == -3 and append(cos=ok + 4, sin=ok, rows=9) == -5
@@ -355,7 +356,12 @@ def test_the_entry_points_refuse_wrong_tensors(how):
     else:
         refused("pair", ("append",), rope=table)
         refused("rope sin", ("append",), rope=(table, table[:9]))
+        refused("rope cos", ("append",), rope=(table[:0], table[:0]))
+        refused("rope cos must be", ("append",), rope=([1.0], table))
         refused("out", both, out=q[:, :2])
+        for name, which in (("queries", ("append", "attend", "select")), ("k_cache", both), ("v_cache", both), ("out", both), ("pages", ("attend",)),
+                            ("keys", ("append",)), ("values", ("append",)), ("key_bounds", ("append", "select")), ("starts", both)):
+            refused(name + " must be a torch.Tensor", which, **{name: [0]})
     refused("pages must be", ("attend",), pages=pages.long())
     refused("pages must be", ("attend",), pages=pages[:, :2])
     refused("pages must be", ("attend",), pages=pages[..., :0])
