@@ -550,7 +550,7 @@ def cached_attention_plan(B, L, R, Rkv, H, P, W, count=0):
     out = (ctypes.c_int * 5)()
     _check(load_library().fa_cached_attention_plan(_sizes(B, Rkv, H, P, W), L, R, count, out))
     res = dict(zip(("kernel", "waves", "rows", "splits", "workgroups"), out))
-    res["kernel"] = ("few", "many")[res["kernel"]]
+    res["kernel"] = ("few", "many", "joined")[res["kernel"]]
     return res
 
 

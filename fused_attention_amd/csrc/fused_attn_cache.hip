@@ -121,6 +121,7 @@ hipError_t for_type(int64_t H, bool bf, F f) {
 // How cached_attention is launched.
 struct AttendPlan {
     bool wide;             // the kernel for many rows
+    bool shared;           // the lists of several tokens joined
     int nq, waves;         // the other one: blocks of 16 query rows and waves of a workgroup
     int64_t tiles, splits, wgs;
 };
@@ -187,15 +188,37 @@ Estimate wide_us(const View& p, int64_t base, int64_t most_keys, float keys, int
     return best;
 }
 
+// How often a page that one of `tokens` lists names is in them all, were they drawn by chance from the whole table: lists of
+// neighbours have more in common, so that joining them gains more than this says.  (4 query heads to each of 8 key heads of 128,
+// 500 tokens, 48 of 250 pages each: 1.34 by chance, 90 us instead of 110; lists that are half alike 59, equal ones 34.  2000 tokens,
+// 32 pages: 1.21 by chance, 454 instead of 439, half alike 299.  With 256 tiles of four waves: 1.9 by chance, 37 instead
+// of 38, half alike 25.  With 192 tiles 27 instead of 20, with 544 and 1.14 by chance 52 instead of 43.)
+double overlap(const View& p, int64_t tokens, int64_t count) {
+    const double listed = count < p.W ? (double)count / p.W : 1.0;
+    return tokens * listed / (1.0 - std::pow(1.0 - listed, (double)tokens));
+}
+
 AttendPlan plan_attend(const View& p, int64_t count, int64_t H) {
     AttendPlan a;
     const int64_t rows = (int64_t)p.L * p.group, heads = (int64_t)p.B * p.Rkv;
     const int64_t most_keys = (count > 0 ? count : (int64_t)p.W) << p.log2_p, steps = ceil_div(most_keys, 64);
     a.wide = false;
+    a.shared = false;
     a.nq = count > 0 || rows <= 16 ? 1 : 2;
     a.tiles = count > 0 ? p.L * ceil_div(p.group, 16) : ceil_div(rows, 16 * a.nq);
     a.waves = fa::cache::kAttendWaves;
     a.splits = 1;
+    if (count > 0 && p.group <= 8 && p.W <= fa::cache::kMostShared) {
+        const int64_t together = fa::cache::shared_tokens(p.group) < p.L ? fa::cache::shared_tokens(p.group) : p.L, tiles = ceil_div(p.L, together);
+        const bool many = heads * tiles >= 3 * kNumCu;   // that fill the chip with two waves each
+        if (heads * tiles >= kNumCu && overlap(p, together, count) >= (many ? 1.1 : 1.5)) {
+            a.shared = true;
+            a.tiles = tiles;
+            a.waves = many ? 2 : fa::cache::kAttendWaves;
+            a.wgs = heads * a.tiles;
+            return a;
+        }
+    }
     const Estimate parts = narrow_splits(p, heads * a.tiles, steps, H);
     if (count > 0 && heads * a.tiles > 4 * kNumCu)
         a.waves = 1;                                     // a wave a tile, nothing to merge: 143 us where four take 152
@@ -364,23 +387,24 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
         using namespace fa::cache;
         constexpr int threads = 64 * kAttendWaves;
         hipError_t e;
-        const int list = (int)count * 4;
         if (a.wide) {
             auto kernel = cached_attention_wide_kernel<h(), b()>;
             e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
             if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
         } else if (count > 0) {
-            const void* kernel = a.waves == 8   ? reinterpret_cast<const void*>(cached_attention_kernel<h(), b(), 1, 8, true>)
-                                 : a.waves == 1 ? reinterpret_cast<const void*>(cached_attention_kernel<h(), b(), 1, 1, true>)
-                                                : reinterpret_cast<const void*>(cached_attention_kernel<h(), b(), 1, kAttendWaves, true>);
-            e = allow_large_lds(kernel, kMostSelected * 4);      // beside up to 64 KiB of its own
-            if (e != hipSuccess) return e;
-            e = a.waves == 8 ? launch(cached_attention_kernel<h(), b(), 1, 8, true>, a.wgs, 512, p, list, s) : a.waves == 1 ? launch(cached_attention_kernel<h(), b(), 1, 1, true>, a.wgs, 64, p, list, s)
-                             : launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, true>, a.wgs, threads, p, list, s);
+            auto kernel = a.shared       ? (a.waves == 2 ? cached_attention_kernel<h(), b(), 1, 2, kShared> : cached_attention_kernel<h(), b(), 1, kAttendWaves, kShared>)
+                          : a.waves == 8 ? cached_attention_kernel<h(), b(), 1, 8, kListed>
+                          : a.waves == 1 ? cached_attention_kernel<h(), b(), 1, 1, kListed>
+                                         : cached_attention_kernel<h(), b(), 1, kAttendWaves, kListed>;
+            // a list; joined: two bytes a page of the table, and the pages that are listed (beside up to 64 KiB of the kernel's own)
+            const int64_t joined = shared_tokens(p.group) * count;
+            const int lds = 4 * (int)(a.shared ? (p.W + 1) / 2 + (joined < p.W ? joined : p.W) : count);
+            e = allow_large_lds(reinterpret_cast<const void*>(kernel), a.shared ? 6 * kMostShared : 4 * kMostSelected);
+            if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * a.waves, p, lds, s);
         } else if (a.nq == 1) {
-            e = launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, false>, a.wgs, threads, p, 0, s);
+            e = launch(cached_attention_kernel<h(), b(), 1, kAttendWaves, kEvery>, a.wgs, threads, p, 0, s);
         } else {
-            e = launch(cached_attention_kernel<h(), b(), 2, kAttendWaves, false>, a.wgs, threads, p, 0, s);
+            e = launch(cached_attention_kernel<h(), b(), 2, kAttendWaves, kEvery>, a.wgs, threads, p, 0, s);
         }
         if (e != hipSuccess || a.splits == 1) return e;
         return launch(cached_attention_join_kernel<h(), b()>, ceil_div(rows, 4), 256, p, 0, s);
@@ -396,7 +420,7 @@ int fa_cached_attention_plan(const fa_cache* cache, int64_t L, int64_t R, int64_
     if (rc != FA_OK) return rc;
     const AttendPlan a = plan_attend(p, count, cache->head_dim);
     if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
-    plan[0] = a.wide;
+    plan[0] = a.wide ? 1 : a.shared ? 2 : 0;
     plan[1] = a.waves;
     plan[2] = a.wide ? fa::cache::kWideRows : 16 * a.nq;
     plan[3] = (int)a.splits;

@@ -312,8 +312,8 @@ int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, in
 /*
  * The launches that fa_cached_attention and fa_select_pages would make for these sizes, without making them (no GPU is touched; only
  * the sizes in `cache` are looked at): for tests of the launcher and for tuning.  fa_cached_attention_plan fills
- * plan[0..4] with: 0 = the kernel for few rows, 1 = the one for many; waves per workgroup; query rows per workgroup; parts
- * that a row's keys are cut into; workgroups.  fa_select_pages_plan fills plan[0..2] with: tokens per workgroup; waves per
+ * plan[0..4] with: 0 = the kernel for few rows, 1 = the one for many, 2 = that for few with the lists of several tokens joined;
+ * waves per workgroup; query rows per workgroup; parts that a row's keys are cut into; workgroups.  fa_select_pages_plan fills plan[0..2] with: tokens per workgroup; waves per
  * workgroup; workgroups.
  */
 int fa_cached_attention_plan(const fa_cache* cache, int64_t L, int64_t R, int64_t count, int* plan);

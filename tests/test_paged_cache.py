@@ -560,12 +560,15 @@ def test_launches_are_within_what_the_kernels_take():
         count = rng.choice([0, 0, 0, rng.randint(1, 4096)])
         plan = capi.cached_attention_plan(B, L, Rkv * group, Rkv, H, P, W, count)
         rows = plan["rows"]
-        tiles = L * -(-group // rows) if count else -(-L * group // rows)
+        joined = plan["kernel"] == "joined"
+        tiles = -(-L // min(L, 16 // group)) if joined else L * -(-group // rows) if count else -(-L * group // rows)
         keys = (count or W) * P
         assert plan["workgroups"] == B * Rkv * tiles * plan["splits"]
         assert 1 <= plan["splits"] <= 64 and (plan["splits"] - 1) * 64 < keys
         if plan["kernel"] == "many":
             assert (plan["waves"], rows) == (8, 256) and not count
+        elif joined:
+            assert count and L > 1 and group <= 8 and W <= 8192 and plan["waves"] in (2, 4) and (rows, plan["splits"]) == (16, 1)
         else:
             assert plan["waves"] == 4 or (count and plan["waves"] in (1, 8))
             assert rows in (16, 32) and (rows == 16 or (L * group > 16 and not count))
@@ -575,7 +578,7 @@ def test_launches_are_within_what_the_kernels_take():
             assert plan["workgroups"] == B * Rkv * -(-L // plan["tokens"])
             assert plan["tokens"] == 1 or (plan["tokens"] * group == 16 and plan["tokens"] * W <= 8192 and plan["waves"] == 4)
             kinds.add(("select", plan["tokens"] > 1, plan["waves"]))
-    assert len(kinds) == 6 + 2 + 3, kinds                         # few rows, many rows, selections
+    assert len(kinds) == 6 + 2 + 2 + 3, kinds                     # few rows, many rows, joined lists, selections
 
 
 def _compare_attention(gpu, B, dtype, H, P, R, Rkv, L, W, layout, causal):
@@ -771,6 +774,37 @@ def test_lists_of_pages_as_they_come(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,R,Rkv,L,H,P,W,count,waves,causal,layout", [
+    (4, 8, 8, 128, 64, 16, 9, 3, 4, True, "blf"), (8, 80, 16, 7, 128, 16, 9, 6, 4, True, "blf"), (8, 16, 16, 100, 16, 16, 7, 2, 2, True, "bhld"),
+    (3, 32, 4, 90, 32, 32, 5, 4, 4, False, "blf"), (4, 24, 8, 150, 128, 16, 12, 5, 2, True, "blf"), (16, 32, 16, 40, 128, 64, 3, 1, 2, False, "bhld"),
+    (6, 24, 12, 90, 64, 128, 2, 2, 2, True, "blf"), (4, 32, 16, 35, 16, 32, 130, 70, 4, True, "blf"),
+])
+@pytest.mark.parametrize("nan", [False, True])
+def test_joined_lists(gpu, dtype, B, R, Rkv, L, H, P, W, count, waves, causal, layout, nan):
+    # lists of several tokens in one tile: repeats, gaps, numbers outside the table, tokens that do not exist, and values that are not
+    # numbers on pages that some of the tokens list
+    p = Problem(B=B, L=L, R=R, Rkv=Rkv, H=H, P=P, W=W, dtype=dtype, seed=H + L + count, layout=layout)
+    plan = capi.cached_attention_plan(B, L, R, Rkv, H, P, W, count)
+    assert (plan["kernel"], plan["waves"]) == ("joined", waves)
+    p.starts = [max(0, W * P - L - 5 * b * b) if b % 3 < 2 else b for b in range(B)]
+    p.lens = [L - (b * L) // (2 * B) for b in range(B)]
+    lists = torch.randint(-1, W + 1, (B, L, Rkv, count), generator=p.gen).to(torch.int32)
+    lists[0, ::2] = lists[0, 0].clone()                  # some alike,
+    lists[-1, 1] = -1                                    # one empty
+    if nan:
+        code = torch.tensor(0x7f, dtype=torch.uint8)
+        p.v_cache.view(torch.uint8)[p.page_table[0, W // 2], 1, 3, H - 1] = code
+        p.k_cache.view(torch.uint8)[p.page_table[0, 0], 0, P - 1, 2] = code + 128
+        p.v_cache.view(torch.uint8)[p.page_table[B - 1, W - 1], :, P - 1] = code
+        p.q[1, 0, 0, 0] = math.nan
+    want = pc.attention(p.cache(), p.q, p.starts, p.lens, selected=lists, causal=causal)
+    assert not nan or (torch.isnan(want[0]).any() and torch.isfinite(want[0]).any())
+    got, lse = _attend(_entries(), p, p.on(gpu), pages=lists.to(gpu), return_lse=True, causal=causal)
+    _check_attention(p, p.by_token(got, R), lse, want)
+
+
+@pytest.mark.gpu
 def test_lists_with_gaps(gpu):
     # a page named on both sides of numbers that name nothing still counts once
     p = Problem(B=2, L=3, R=4, Rkv=2, H=64, P=16, W=6, seed=22)
@@ -796,15 +830,16 @@ def test_the_widest_table_and_the_longest_lists(gpu):
     assert torch.equal(pages.cpu(), want)
     got, lse = _attend(m, p, p.on(gpu), pages=pages, return_lse=True)
     _check_attention(p, p.by_token(got, 2), lse, pc.attention(cache, p.q, p.starts, p.lens, selected=want))
-    for B, L, waves in ((2, 1, 4), (100, 1, 8), (3, 200, 1)):
-        p = Problem(B=B, L=L, R=2, Rkv=2, H=128, P=16, W=16, seed=21)
-        assert capi.cached_attention_plan(B, L, 2, 2, 128, 16, 16, 4096)["waves"] == waves
+    for B, L, R, kernel, waves in ((2, 1, 2, "few", 4), (100, 1, 2, "few", 8), (3, 200, 18, "few", 1), (4, 100, 16, "joined", 4), (4, 200, 16, "joined", 2)):
+        p = Problem(B=B, L=L, R=R, Rkv=2, H=128, P=16, W=16, seed=21)
+        plan = capi.cached_attention_plan(B, L, R, 2, 128, 16, 16, 4096)
+        assert (plan["kernel"], plan["waves"]) == (kernel, waves)
         p.starts = [(31 * b) % (256 - L + 1) for b in range(B)]
         lists = torch.full((B, L, 2, 4096), -1, dtype=torch.int32)
         lists[..., 5], lists[..., 100], lists[..., 101], lists[..., 4095] = 3, 9, 3, 0
         want = pc.attention(p.cache(), p.q, p.starts, p.lens, selected=lists)
         got, lse = _attend(m, p, p.on(gpu), pages=lists.to(gpu), return_lse=True)
-        _check_attention(p, p.by_token(got, 2), lse, want)
+        _check_attention(p, p.by_token(got, R), lse, want)
 
 
 @pytest.mark.gpu
