@@ -174,13 +174,19 @@ float narrow_us(const View& p, int64_t base, float keys, int64_t steps, int64_t 
 }
 
 // The wide kernel: the longest workgroup's tiles of 64 keys, or what the chip's workgroups take in all, of which a compute
-// unit holds one at head_dim 128 and two below.  (The same three: 43, 40 us; 98, 98 in four parts; 145, 172.)
-Estimate wide_us(const View& p, int64_t base, int64_t most_keys, float keys, int64_t H) {
+// unit holds one at head_dim 128 and two or three below.  With one block of 16 rows a wave instead of two a tile takes 0.6 of the time and
+// there are twice as many workgroups: for calls that the longest workgroup bounds.  (The same three, measured with two blocks
+// and with one: 38, 33 us; 94 in four parts, 107 in two; 178, 199.  1500 tokens, 32 heads on 8 of 128: 57, 41; 512 tokens of 4 times 16
+// heads of 64: 21, 16, and 18 by the other kernel; 2048 tokens behind 14336, 32 heads on 8 of 128: 519, 661.)
+Estimate wide_us(const View& p, int64_t nq, int64_t most_keys, float keys, int64_t H) {
     Estimate best{1, 3.0e38f};
+    const int64_t base = (int64_t)p.B * p.Rkv * ceil_div((int64_t)p.L * p.group, fa::cache::kWideWaves * 16 * nq);
     for (int64_t s = 1; s <= kMostSplits && (s == 1 || (base * s <= 4 * kNumCu && s * fa::cache::kWideKeys < most_keys)); ++s) {
         const float per_cu = (float)(base * s) / kNumCu;
-        const float tile = H > 64 ? 2.17f : (per_cu > 1.f ? 2.3f : 1.6f) - (H > 32 ? 0.f : 0.3f);
-        const float all = H > 64 ? 2.17f * (float)ceil_div(base * s, kNumCu) : 1.15f * per_cu;
+        const float two = H > 64 ? 2.17f : (per_cu > 1.f ? 2.3f : 1.6f) - (H > 32 ? 0.f : 0.3f);
+        const float one = H > 64 ? 1.33f : H > 32 ? (per_cu > 1.f ? 1.65f : 1.17f) : (per_cu > 1.f ? 1.2f : 0.95f);
+        const float tile = nq == 2 ? two : one;
+        const float all = H > 64 ? tile * (float)ceil_div(base * s, kNumCu) : (nq == 2 ? 1.3f : 0.75f) * per_cu;
         const float longest = tile * (float)ceil_div(most_keys, s * fa::cache::kWideKeys), whole = all * keys / (float)(s * fa::cache::kWideKeys);
         const float us = 6.f + (longest > whole ? longest : whole) + join_us(p, s, H);
         if (us < best.us) best = {s, us};
@@ -228,13 +234,14 @@ AttendPlan plan_attend(const View& p, int64_t count, int64_t H) {
     if (count > 0 && heads * a.tiles <= kNumCu && a.splits <= 2) a.waves = 8, a.splits = 1;
     if (count == 0 && rows > 32) {
         const float keys = most_keys > p.L ? (float)most_keys - 0.5f * (float)p.L : 0.5f * (float)most_keys;
-        const int64_t tiles = ceil_div(rows, fa::cache::kWideRows);
-        const Estimate wide = wide_us(p, heads * tiles, most_keys, keys, H);
+        const Estimate two = wide_us(p, 2, most_keys, keys, H), one = wide_us(p, 1, most_keys, keys, H), wide = one.us < two.us ? one : two;
+        const int nq = one.us < two.us ? 1 : 2;
         const float narrow = a.splits > 1 ? parts.us + 6.f : narrow_us(p, heads * a.tiles, keys, steps, H);
         if (wide.us < narrow) {
+            a.nq = nq;
             a.wide = true;
             a.waves = fa::cache::kWideWaves;
-            a.tiles = tiles;
+            a.tiles = ceil_div(rows, fa::cache::kWideWaves * 16 * nq);
             a.splits = wide.splits;
         }
     }
@@ -388,7 +395,7 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
         constexpr int threads = 64 * kAttendWaves;
         hipError_t e;
         if (a.wide) {
-            auto kernel = cached_attention_wide_kernel<h(), b()>;
+            auto kernel = a.nq == 1 ? cached_attention_wide_kernel<h(), b(), 1> : cached_attention_wide_kernel<h(), b(), 2>;
             e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
             if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
         } else if (count > 0) {
@@ -422,7 +429,7 @@ int fa_cached_attention_plan(const fa_cache* cache, int64_t L, int64_t R, int64_
     if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
     plan[0] = a.wide ? 1 : a.shared ? 2 : 0;
     plan[1] = a.waves;
-    plan[2] = a.wide ? fa::cache::kWideRows : 16 * a.nq;
+    plan[2] = 16 * a.nq * (a.wide ? fa::cache::kWideWaves : 1);
     plan[3] = (int)a.splits;
     plan[4] = (int)a.wgs;
     return FA_OK;
