@@ -163,30 +163,33 @@ Estimate narrow_splits(const View& p, int64_t base, int64_t steps, int64_t H) {
 }
 
 // Many rows, the narrow kernel in one part: rounds of the workgroups that a chip holds, and what the products and exponentials
-// take in all; or the longest workgroup.  (fp16, causal, estimated and measured: 8 sequences of 1000 tokens of 12 heads of 64: 46, 51 us; 2000 rows
+// take in all; or the longest workgroup; or the codes, which every row tile reads, where they are more than the second-level caches
+// hold (8 tokens of 64 sequences of 1000, 40 heads on 8 of 128: 58 us, 55).  (fp16, causal, estimated and measured: 8 sequences of 1000 tokens of 12 heads of 64: 46, 51 us; 2000 rows
 // of each of 8 heads of 128 over 8000 tokens: 94, 99; 4096 tokens of 32 heads of 128: 251, 247.)
 float narrow_us(const View& p, int64_t base, float keys, int64_t steps, int64_t H) {
     const int64_t resident = H > 64 ? 2 * kNumCu : 3 * kNumCu;
-    const float rate = H > 64 ? 1.5e6f : H > 32 ? 2.4e6f : 3.e6f;       // rows times keys
-    const float whole = (H > 64 ? 9.f : 6.5f) * (float)ceil_div(base, resident) + (float)p.B * (float)p.L * (float)p.R * keys / rate;
+    const float rate = H > 64 ? 1.5e6f : H > 32 ? 2.4e6f : 3.e6f;       // rows times keys; the rows of whole tiles
+    const float whole = (H > 64 ? 9.f : 6.5f) * (float)ceil_div(base, resident) + (float)base * 32.f * keys / rate;
     const float longest = 6.f + (1.f + 0.009f * (float)H) * (float)ceil_div(steps, fa::cache::kAttendWaves);
-    return whole > longest ? whole : longest;
+    const float us = whole > longest ? whole : longest;
+    const float bytes = (float)p.B * (float)p.Rkv * keys * 2.f * (float)H, read = 6.f + (float)base / ((float)p.B * (float)p.Rkv) * bytes / 5.e6f;
+    return bytes > 3.2e7f && read > us ? read : us;
 }
 
 // The wide kernel: the longest workgroup's tiles of 64 keys, or what the chip's workgroups take in all, of which a compute
-// unit holds one at head_dim 128 and two or three below.  With one block of 16 rows a wave instead of two a tile takes 0.6 of the time and
-// there are twice as many workgroups: for calls that the longest workgroup bounds.  (The same three, measured with two blocks
-// and with one: 38, 33 us; 94 in four parts, 107 in two; 178, 199.  1500 tokens, 32 heads on 8 of 128: 57, 41; 512 tokens of 4 times 16
-// heads of 64: 21, 16, and 18 by the other kernel; 2048 tokens behind 14336, 32 heads on 8 of 128: 519, 661.)
+// unit holds one at head_dim 128 and two below; with one block of 16 rows a wave instead of two, two and three.  Then a tile
+// takes 0.6 of the time and there are twice as many workgroups: for calls that the longest workgroup bounds.  (The same three,
+// measured with two blocks and with one: 38, 33 us; 90, 91, each in four parts; 178, 199.  32 heads on 8 of 128: 1500 tokens 57, 43, by
+// the other kernel 59; 2048 behind 14336 515, 528.  8 tokens of 64 sequences of 1000, 40 heads on 8 of 128: 66, 33, by the other 55.)
 Estimate wide_us(const View& p, int64_t nq, int64_t most_keys, float keys, int64_t H) {
     Estimate best{1, 3.0e38f};
     const int64_t base = (int64_t)p.B * p.Rkv * ceil_div((int64_t)p.L * p.group, fa::cache::kWideWaves * 16 * nq);
     for (int64_t s = 1; s <= kMostSplits && (s == 1 || (base * s <= 4 * kNumCu && s * fa::cache::kWideKeys < most_keys)); ++s) {
         const float per_cu = (float)(base * s) / kNumCu;
-        const float two = H > 64 ? 2.17f : (per_cu > 1.f ? 2.3f : 1.6f) - (H > 32 ? 0.f : 0.3f);
-        const float one = H > 64 ? 1.33f : H > 32 ? (per_cu > 1.f ? 1.65f : 1.17f) : (per_cu > 1.f ? 1.2f : 0.95f);
+        const float two = H > 64 ? 2.02f : (per_cu > 1.f ? 2.3f : 1.6f) - (H > 32 ? 0.f : 0.3f);
+        const float one = H > 64 ? 1.36f + (per_cu > 1.f ? 0.4f * ((per_cu < 2.f ? per_cu : 2.f) - 1.f) : 0.f) : H > 32 ? (per_cu > 1.f ? 1.65f : 1.17f) : (per_cu > 1.f ? 1.2f : 0.95f);
         const float tile = nq == 2 ? two : one;
-        const float all = H > 64 ? tile * (float)ceil_div(base * s, kNumCu) : (nq == 2 ? 1.3f : 0.75f) * per_cu;
+        const float all = nq == 1 ? (H > 64 ? 1.12f : 0.75f) * per_cu : H > 64 ? tile * (float)ceil_div(base * s, kNumCu) : 1.3f * per_cu;
         const float longest = tile * (float)ceil_div(most_keys, s * fa::cache::kWideKeys), whole = all * keys / (float)(s * fa::cache::kWideKeys);
         const float us = 6.f + (longest > whole ? longest : whole) + join_us(p, s, H);
         if (us < best.us) best = {s, us};
@@ -396,8 +399,9 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
         hipError_t e;
         if (a.wide) {
             auto kernel = a.nq == 1 ? cached_attention_wide_kernel<h(), b(), 1> : cached_attention_wide_kernel<h(), b(), 2>;
-            e = allow_large_lds(reinterpret_cast<const void*>(kernel), wide_lds_bytes<h()>());
-            if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, wide_lds_bytes<h()>(), s);
+            const int lds = a.nq == 1 ? wide_lds_bytes<h(), 1>() : wide_lds_bytes<h(), 2>();
+            e = allow_large_lds(reinterpret_cast<const void*>(kernel), lds);
+            if (e == hipSuccess) e = launch(kernel, a.wgs, 64 * kWideWaves, p, lds, s);
         } else if (count > 0) {
             auto kernel = a.shared       ? (a.waves == 2 ? cached_attention_kernel<h(), b(), 1, 2, kShared> : cached_attention_kernel<h(), b(), 1, kAttendWaves, kShared>)
                           : a.waves == 8 ? cached_attention_kernel<h(), b(), 1, 8, kListed>
