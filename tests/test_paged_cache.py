@@ -846,6 +846,28 @@ def test_the_widest_table_and_the_longest_lists(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("L,W,waves", [(512, 8192, 4), (1536, 8191, 2)])
+def test_joined_lists_of_the_longest_tables(gpu, L, W, waves):
+    # queries of zero give every key one weight, so that the log-sum-exp counts the keys that a row's list names: a page more or less
+    # among some 3200 moves it by 2^-12, rounding by 2^-18 at most: the sum of n weights of 2^7 is exact below 2^24, its logarithm of
+    # base 2, below 24, is off by 2^-20 and its product with ln 2 by 2^-20
+    p = Problem(B=1, L=L, R=8, Rkv=8, H=16, P=16, W=W, dtype=torch.bfloat16, seed=24, extra=0, bounds=False)
+    plan = capi.cached_attention_plan(1, L, 8, 8, 16, 16, W, 4096)
+    assert (plan["kernel"], plan["waves"]) == ("joined", waves)
+    p.q = torch.zeros_like(p.q)
+    p.starts = [16 * W - L]
+    lists = torch.randint(-1, W + 1, (1, L, 8, 4096), generator=p.gen).to(torch.int32).to(gpu)
+    got, lse = _attend(_entries(), p, p.on(gpu), pages=lists, return_lse=True)
+    named = torch.zeros(L, 8, W + 2, dtype=torch.bool, device=gpu)
+    named.scatter_(2, lists[0].long() + 1, True)
+    limit = p.starts[0] + 1 + torch.arange(L, device=gpu)
+    seen = (limit[:, None] - 16 * torch.arange(W, device=gpu)).clamp(0, 16)
+    n = torch.stack([(named[:, head, 1:-1] * seen).sum(-1) for head in range(8)], 0).double()
+    assert (lse[0].double() - n.log()).abs().max().item() < 2.0 ** -14
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.gpu
 def test_pages_beyond_32_bits_of_bytes(gpu):
     # a cache of 5 GB for keys and for values each, its last pages in use
     m = _entries()
