@@ -4,6 +4,8 @@
 
 #include "../../include/fused_attn.h"
 
+#include <algorithm>
+#include <array>
 #include <cmath>
 #include <mutex>
 #include <utility>
@@ -78,10 +80,20 @@ int check_strided(const void* t, const Strides3& s, int64_t B, int64_t heads, in
     return FA_OK;
 }
 
-// What is written: the same, with a place of its own for every row.
+// What is written: the same, with a place of its own for every row.  Of the dimensions with more than one element, by their strides,
+// each has to step over all the rows that those before it place.
 int check_written(const void* t, const Strides3& s, int64_t B, int64_t heads, int64_t L, int64_t H) {
-    if ((s.b == 0 && B > 1) || (s.h == 0 && heads > 1)) return FA_ERR_BAD_STRIDE;
-    return check_strided(t, s, B, heads, L, H);
+    const int rc = check_strided(t, s, B, heads, L, H);
+    if (rc != FA_OK) return rc;
+    std::array<std::pair<int64_t, int64_t>, 3> dims = {{{s.b, B}, {s.h, heads}, {s.l, L}}};
+    std::sort(dims.begin(), dims.end());
+    uint64_t taken = (uint64_t)H;                        // three products below kMaxElems fit
+    for (const auto& [stride, n] : dims) {
+        if (n == 1) continue;
+        if ((uint64_t)stride < taken) return FA_ERR_BAD_STRIDE;
+        taken += (uint64_t)stride * (uint64_t)(n - 1);
+    }
+    return FA_OK;
 }
 
 // Dynamic LDS above 64 KiB has to be opted into per kernel function and per device.

@@ -631,7 +631,7 @@ const char* fa_strerror(int status) {
         case FA_ERR_BAD_SHAPE:
             return "fa_fwd: B, R and L must be at least 1 (fa_qkv_proj: and the feature counts multiples of 64; fa_cache: and every size, R a multiple of heads)";
         case FA_ERR_BAD_STRIDE:
-            return "fa_fwd: strides must be non-negative multiples of 8 elements and stride_l >= head_dim";
+            return "fa_fwd: strides must be non-negative multiples of 8 elements and stride_l >= head_dim (fa_cache: and rows that are written apart)";
         case FA_ERR_MISALIGNED: return "fa_fwd: q, k, v and out must be 16-byte aligned (fa_cache: and keys, values, key_bounds, rope tables and workspace)";
         case FA_ERR_TOO_LARGE: return "fa_fwd: problem size exceeds the supported index range";
         case FA_ERR_BAD_FLAGS: return "fa_fwd_ex: unknown flag, or FA_FLAG_CAUSAL together with a mask";

@@ -261,7 +261,9 @@ typedef struct fa_cache {
  * A page that a call writes must belong to one sequence and stand once in its table.
  * q (nullable, strides q_stride_*, R heads) is rotated likewise into q_out (strides out_stride_*, not overlapping q),
  * rounded once; rows of tokens that do not exist, or from rope_rows on, become zeros.  R is not looked at without q.
- * Strides of 0 are for k, v and q only (FA_ERR_BAD_STRIDE for q_out, here, and out, below).
+ * What is written (q_out here, out below) has a place of its own for every row: of its dimensions with more than one element, in
+ * the order of their strides, each steps over all the rows that those before it place (FA_ERR_BAD_STRIDE otherwise; strides of 0 and
+ * rows that overlap are for k, v and q only).
  */
 int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t kv_stride_b, int64_t kv_stride_h, int64_t kv_stride_l,
                     const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,

@@ -270,6 +270,39 @@ def test_the_library_refuses_what_its_header_says():
     assert "page_size" in capi.strerror(-9) and "workspace" in capi.strerror(-10)
 
 
+def test_outputs_whose_rows_overlap_are_refused():
+    # by zero strides, by strides that are too small, between any two dimensions; rows that lie apart are not: with nothing else wrong
+    # those calls fail later, at the workspace that they lack
+    lib = capi.load_library()
+    ok = 0x1000                                                    # never dereferenced
+    # one long table and few rows: the keys are in parts, which need a workspace
+    c = capi.Cache(keys=ok, values=ok, key_exponents=ok, value_exponents=ok, key_bounds=ok, page_table=ok, pages=10, heads=2, page_size=64,
+                   head_dim=64, sequences=3, table_width=4096, table_stride=4096)
+
+    def attend(os, L=2, R=4, sequences=3):
+        c.sequences = sequences
+        return lib.fa_cached_attention(ctypes.byref(c), ok, 512, 64, 256, ok, *os, None, None, 0, ok, None, L, R, 0.125, 0, None, 0, None)
+
+    def append(os, L=2, R=4):
+        c.sequences = 3
+        # a flag of the rotation that is out of order behind the strides
+        return lib.fa_cache_append(ctypes.byref(c), ok, ok, 512, 64, 128, ok, 512, 64, 256, ok, *os, ok, None, L, R, ok, None, 9, 0, None)
+
+    apart = [(512, 64, 256), (512, 128, 64), (64, 384, 192), (4096, 1024, 64), (128, 64 * 12, 64), (64, 64 * 6, 64 * 3), (520, 64, 256),
+             (520, 64, 264)]
+    overlapping = [(512, 8, 256), (8, 64, 256), (504, 64, 256), (512, 56, 256), (512, 64, 248), (512, 64, 64), (64, 64, 256), (256, 64, 256),
+                   (512, 120, 64), (448, 128, 64), (0, 64, 256), (512, 0, 256), (64, 384, 184), (512, 64, 264), (2 ** 60, 2 ** 60, 2 ** 59)]
+    for os in apart:
+        assert attend(os) == -10 and append(os) == -1, os
+    for os in overlapping:
+        assert attend(os) == -4 and append(os) == -4, os
+    # a dimension of one element places nothing
+    assert attend((0, 64, 256), sequences=1) == -10 and attend((8, 64, 256), sequences=1) == -10
+    assert attend((256, 64, 64), L=1) == -10 and attend((192, 64, 64), L=1) == -4
+    c.heads = 1
+    assert attend((128, 0, 64), R=1) == -10 and attend((64, 8, 64), R=1) == -4
+
+
 def _entries():
     import fused_attn
 
