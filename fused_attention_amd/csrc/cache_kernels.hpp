@@ -89,6 +89,13 @@ __device__ __forceinline__ float quad_sum(float x) {
     return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
 }
 
+// Between LDS accesses of the lanes of one wave to each other's places.  LDS serves a wave in order, so that nothing has to wait: this
+// keeps the compiler from exchanging them, and is no instruction.
+__device__ __forceinline__ void lanes_in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }   // e in [-126, 127]
 

@@ -126,3 +126,44 @@ int main() {
     subprocess.run([HIPCC] + build.HIPCC_FLAGS + [str(tmp_path / "div.hip"), "-o", str(tmp_path / "div")], check=True, capture_output=True)
     ran = subprocess.run([str(tmp_path / "div")], capture_output=True, text=True)
     assert ran.returncode == 0, ran.stdout
+
+
+# (kernel, template arguments): keys through LDS in each width and form of the rows; histograms of one wave
+CACHE_KERNELS = [("cached_attention_kernel", "%d, %s, %d, %d, fa::cache::%s" % at) for at in (
+    (32, "false", 1, 4, "kEvery"), (64, "true", 2, 4, "kEvery"), (128, "false", 1, 8, "kListed"), (128, "true", 1, 1, "kListed"),
+    (64, "false", 1, 2, "kShared"))] + [("select_pages_rows_kernel", "64, false")]
+
+
+def test_lanes_that_exchange_through_lds_do_so_in_order(tmp_path):
+    # Where the lanes of a wave read what others of it wrote, no instruction is needed between, but the compiler must not exchange the
+    # two either: between stores, counts and loads there is a barrier, of the workgroup or of the wave.
+    if not os.path.exists(HIPCC):
+        pytest.skip("no hipcc")
+    params = {"cached_attention_kernel": "AttendParams", "select_pages_rows_kernel": "SelectParams"}
+    source = ['#include "%s"' % os.path.join(build.CSRC, "cache_kernels.hpp")]
+    source += ["template __global__ void fa::cache::%s<%s>(const fa::cache::%s);" % (name, at, params[name]) for name, at in CACHE_KERNELS]
+    (tmp_path / "cache.hip").write_text("\n".join(source) + "\n")
+    subprocess.run([HIPCC] + build.HIPCC_FLAGS + ["--cuda-device-only", "-S", str(tmp_path / "cache.hip"), "-o", str(tmp_path / "cache.s")],
+                   check=True, capture_output=True)
+    checked = 0
+    kernel = last = None
+    by_wave = False
+    for line in (tmp_path / "cache.s").read_text().splitlines():
+        found = re.match(r"_ZN2fa5cache\d+(cached_attention_kernel|select_pages_rows_kernel)\w+:", line)
+        if found:
+            kernel, last, by_wave = line, None, False
+        elif line.startswith(".Lfunc_end"):
+            checked += kernel is not None and by_wave
+            kernel = None
+        elif kernel is not None:
+            text = line.strip()
+            if "s_barrier" in text or "wave barrier" in text:
+                last = None
+                by_wave = by_wave or "wave barrier" in text
+            # the exchanged ones: keys and the histogram's words, 8 or 16 bytes at a time, and its counts
+            op = re.match(r"ds_(read_b64|read_b128|write_b64|write_b128|add_u32)", text)
+            if op:
+                kind = op.group(1).split("_")[0]
+                assert last in (None, kind), (kernel, text)
+                last = kind
+    assert checked == len(CACHE_KERNELS)
