@@ -219,8 +219,9 @@ int fa_qkv_proj_variant(int64_t B, int64_t L, int64_t F_in, int64_t R, int64_t H
  *   keys, values     [pages, heads, page_size, head_dim], one e4m3 code (OCP FP8: torch.float8_e4m3fn) per value
  *   key_exponents, value_exponents
  *                    int8 [pages, heads]: a code c of the page and head stands for c * 2^exponent
- *   key_bounds       (nullable) int8 [pages, heads, 2, head_dim]: the largest and the smallest key of each channel of the page,
- *                    in steps of 2^(key exponent + 2), rounded upwards and downwards; what fa_select_pages reads
+ *   key_bounds       (nullable) int8 [pages, heads, 2, head_dim]: the largest and the smallest key of each channel of the page, as
+ *                    appended (rotated, before the rounding to e4m3), in steps of 2^(key exponent + 2), rounded upwards and
+ *                    downwards; what fa_select_pages reads
  *   page_table       int32 [sequences, table_width], rows table_stride elements apart: the page of the tokens
  *                    w * page_size .. (w + 1) * page_size - 1 of a sequence; a number outside [0, pages) is no page
  *
@@ -302,8 +303,9 @@ int64_t fa_cached_attention_workspace(const fa_cache* cache, int64_t L, int64_t 
  * the pages up to the one of the token itself, which is always taken; of the others those with the largest
  *   2^(key exponent) * max over the key head's query heads of  sum_d max(q8_d, 0) * largest_d + min(q8_d, 0) * smallest_d
  * where q8 = round(q * 2^-e) with the smallest e that keeps the group's queries within 127 (not finite: 0), and largest and
- * smallest are the cache's key_bounds: an upper bound, up to the rounding of q, of what a key of the page can score.  Whole
- * numbers throughout; equal scores go to the lowest place.  Tokens that do not exist get -1 only.
+ * smallest are the cache's key_bounds: 2^-(e + 2) times an upper bound of what the page's keys score with q8 * 2^e as they were
+ * appended.  What the cache holds of them may score more by the rounding to e4m3: in each channel a code may lie outside its bounds by a
+ * sixteenth of the key (of small keys, 2^-9 of the page's power of two).  Whole numbers throughout; equal scores go to the lowest place.  Tokens that do not exist get -1 only.
  * q as above, rotated already.  cache->keys, values and value_exponents are not looked at.  table_width is at most 32768 and
  * count at most 4096 (FA_ERR_TOO_LARGE).  Needs no workspace.
  */

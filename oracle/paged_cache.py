@@ -9,7 +9,8 @@ What pins each function (tests/test_paged_cache.py, on the CPU):
   exponent_of  against its definition at every border 448 * 2^e and its neighbours
   append       what was appended comes back within half a step of e4m3; parts give what the whole gives
   attention    against `oracle.attention` on the values that the cache stands for
-  select       the score of a page is no smaller than what any of its keys scores with the rounded query, and closed forms
+  select       the score of a page is no smaller than what any of its keys scores with the rounded query, as appended, nor by more than
+               the rounding to e4m3 smaller than what the stored ones do, and closed forms
 """
 import math
 

@@ -199,6 +199,42 @@ def test_selection_of_the_oracle_bounds_the_scores():
     assert pc.select(cache, p.q, p.starts, p.lens, 3)[0, 0].tolist() == [[0, 1, 5]] * 2
 
 
+@pytest.mark.parametrize("H,P,n", [(32, 16, 96), (64, 64, 150), (16, 128, 128)])
+def test_scores_bound_the_keys_as_appended(H, P, n):
+    # The bounds that appending makes are of the keys before their rounding to e4m3: what was appended lies within, in every channel, and
+    # scores no more with the rounded query than its page.  The codes may lie outside: 433 becomes 448 behind a bound of 436.  By their
+    # rounding alone: half a step, 2^-4 of a normal number or 2^-10, and where exponents grew afterwards up to 2^-10 once more.
+    p = Problem(B=1, L=n, R=4, Rkv=2, H=H, P=P, W=-(-n // P), seed=31)
+    p.k *= torch.linspace(-2, 3, n).exp2()[:, None, None].half()   # exponents grow within pages
+    p.k[0, 3, 0, 2] = 433.0
+    cache = p.cache()
+    first = 0
+    for part in (1, 2, 40, n):                                     # in parts
+        part = min(part, n - first)
+        pc.append(cache, p.k[:, first:first + part], p.v[:, first:first + part], [first], [part])
+        first += part
+    assert first == n
+    outside = 0
+    for w in range(p.W):
+        page, here = cache.page(0, w), p.k[0, w * P:(w + 1) * P].double().numpy()
+        for head in range(2):
+            e = cache.exponents["k"][page, head]
+            keys = here[:, head] * 2.0 ** -e
+            codes = cache.codes["k"][page, head, :len(keys)]
+            up, down = cache.bounds[page, head] * 4.0
+            assert (keys <= up).all() and (keys >= down).all() and (keys.max(0) > up - 4).all() and (keys.min(0) < down + 4).all()
+            slack = np.abs(keys).max(0) * 2.0 ** -4 + 2.0 ** -9
+            assert (codes <= up + slack).all() and (codes >= down - slack).all()
+            outside += (codes > up).sum() + (codes < down).sum()
+            x = p.q[0, 0, 2 * head:2 * head + 2].double().numpy()
+            q8 = np.rint(x * 2.0 ** -math.ceil(math.log2(np.abs(x).max() / 127)))
+            score = (np.maximum(q8, 0) @ up + np.minimum(q8, 0) @ down).max()
+            assert (keys @ q8.T).max() <= score and (codes @ q8.T).max() <= score + (np.abs(q8) @ slack).max()
+    at = cache.page(0, 0)
+    assert cache.exponents["k"][at, 0] == 0 and cache.codes["k"][at, 0, 3, 2] == 448 and cache.bounds[at, 0, 0, 2] * 4 == 436
+    assert outside > 1
+
+
 # ---- refusals, on the CPU ----
 
 def test_the_library_refuses_what_its_header_says():
