@@ -145,12 +145,16 @@ hipError_t allow_large_lds(const void* kernel, int bytes) {
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
-    std::lock_guard<std::mutex> guard(lock);
-    for (const auto& d : done)
-        if (d.first == kernel && d.second == dev) return hipSuccess;
-    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess) done.emplace_back(kernel, dev);
-    return e;
+    try {
+        std::lock_guard<std::mutex> guard(lock);
+        for (const auto& d : done)
+            if (d.first == kernel && d.second == dev) return hipSuccess;
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == hipSuccess) done.emplace_back(kernel, dev);
+        return e;
+    } catch (...) {          // nothing is thrown through a C entry; not remembered, it is asked for again the next time
+        return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    }
 }
 
 // BF selects the bf16 instantiation (namespace fa::bf16) of the same kernel source.

@@ -167,3 +167,73 @@ def test_lanes_that_exchange_through_lds_do_so_in_order(tmp_path):
                 assert last in (None, kind), (kernel, text)
                 last = kind
     assert checked == len(CACHE_KERNELS)
+
+
+def test_no_exception_leaves_a_c_entry(tmp_path):
+    # The host side alone, with a HIP runtime that does nothing and no memory to be had: launches that opt into more LDS and would
+    # remember that they did return a status all the same, every time.
+    if not os.path.exists(HIPCC):
+        pytest.skip("no hipcc")
+    (tmp_path / "main.cpp").write_text(r"""
+#include <cstdio>
+#include <cstdlib>
+#include <new>
+#include "fused_attn.h"
+static bool memory = true;
+static int opted = 0, launched = 0;
+void* operator new(std::size_t n) {
+    void* p = memory ? std::malloc(n) : nullptr;
+    if (p == nullptr) throw std::bad_alloc();
+    return p;
+}
+void operator delete(void* p) noexcept { std::free(p); }
+void operator delete(void* p, std::size_t) noexcept { std::free(p); }
+extern "C" {
+int hipGetDevice(int* d) { *d = 0; return 0; }
+int hipFuncSetAttribute(const void*, int, int) { ++opted; return 0; }
+struct Dim { unsigned x, y, z; };
+int hipLaunchKernel(const void*, Dim, Dim, void**, std::size_t, void*) { ++launched; return 0; }
+void** __hipRegisterFatBinary(const void*) { static void* handle; return &handle; }
+void __hipRegisterFunction(...) {}
+void __hipUnregisterFatBinary(void**) {}
+int __hipPopCallConfiguration(...) { return 0; }
+int hipEventCreate(...) { return 0; }
+int hipEventDestroy(...) { return 0; }
+int hipEventRecord(...) { return 0; }
+int hipEventSynchronize(...) { return 0; }
+int hipEventElapsedTime(...) { return 0; }
+const char* hipGetErrorString(int) { return ""; }
+}
+int main() {
+    alignas(16) static char room[64];
+    const int32_t* n = reinterpret_cast<const int32_t*>(room);
+    fa_cache c = {room, room, room, room, room, n, 1000, 8, 64, 128, 1, 100, 100};
+    for (int i = 0; i < 6; ++i) {
+        memory = i >= 3;
+        const int before = opted;
+        const int many = fa_cached_attention(&c, room, 0, 128, 4096, room, 0, 128, 4096, nullptr, nullptr, 0, n, nullptr, 2000, 32, 1.f, 1,
+                                             room, (int64_t)1 << 40, nullptr);
+        const int listed = fa_cached_attention(&c, room, 0, 128, 4096, room, 0, 128, 4096, nullptr, n, 40, n, nullptr, 2, 32, 1.f, 1,
+                                               room, (int64_t)1 << 40, nullptr);
+        const int select = fa_select_pages(&c, room, 0, 128, 4096, reinterpret_cast<int32_t*>(room), 4, n, nullptr, 1, 32, 0, nullptr);
+        const int dense = fa_fwd(room, room, room, nullptr, room, 8, 32, 4096, 128, 32 * 4096 * 128, 4096 * 128, 128, 0.1f, nullptr);
+        std::printf("%d %d %d %d, %d\n", many, listed, select, dense, opted - before);
+    }
+    std::printf("%d\n", launched);
+}
+""")
+    objects = []
+    for name in build.LIB_SOURCES:
+        objects.append(str(tmp_path / (name + ".o")))
+        subprocess.run([HIPCC, "--offload-arch=gfx950", "-std=c++17", "-O1", "-w", "-fPIC", "--cuda-host-only", "-c", os.path.join(build.CSRC, name), "-o",
+                        objects[-1]], check=True, capture_output=True)
+    subprocess.run(["g++", "-std=c++17", "-w", "-I" + os.path.join(build.REPO_DIR, "include"), str(tmp_path / "main.cpp")] + objects +
+                   ["-Wl,--unresolved-symbols=ignore-in-object-files", "-o", str(tmp_path / "main")], check=True, capture_output=True)
+    ran = subprocess.run([str(tmp_path / "main")], capture_output=True, text=True)
+    assert ran.returncode == 0, ran.stderr
+    lines = ran.stdout.split("\n")
+    statuses, asked = zip(*(line.split(", ") for line in lines[:6]))
+    assert set(statuses) == {"0 0 0 0"}, lines
+    # asked for until there is memory to remember it, and then no more
+    assert min(int(n) for n in asked[:4]) >= 4 and asked[4:] == ("0", "0"), lines
+    assert int(lines[6]) >= 24
