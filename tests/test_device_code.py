@@ -237,3 +237,34 @@ int main() {
     # asked for until there is memory to remember it, and then no more
     assert min(int(n) for n in asked[:4]) >= 4 and asked[4:] == ("0", "0"), lines
     assert int(lines[6]) >= 24
+
+
+def test_the_cache_kernels_keep_their_values_in_registers(tmp_path):
+    # None of their values pass through scratch memory but for those of the lists at head_dim 128 with one and four waves, which are
+    # compiled for three waves a SIMD: at most 16 bytes a lane.
+    if not os.path.exists(HIPCC):
+        pytest.skip("no hipcc")
+    attend = [(h, nq, waves, rows) for h in (64, 128) for nq, waves, rows in (
+        (1, 4, "kEvery"), (2, 4, "kEvery"), (1, 8, "kListed"), (1, 4, "kListed"), (1, 1, "kListed"), (1, 4, "kShared"), (1, 2, "kShared"))]
+
+    def compiled(element):
+        source = ['#include "%s"' % os.path.join(build.CSRC, "cache_kernels.hpp")]
+        source += ["template __global__ void fa::cache::cached_attention_kernel<%d, %s, %d, %d, fa::cache::%s>(const fa::cache::AttendParams);" %
+                   (h, element, nq, waves, rows) for h, nq, waves, rows in attend]
+        source += ["template __global__ void fa::cache::cached_attention_wide_kernel<%d, %s, %d>(const fa::cache::AttendParams);" % (h, element, nq)
+                   for h in (64, 128) for nq in (1, 2)]
+        (tmp_path / (element + ".hip")).write_text("\n".join(source) + "\n")
+        subprocess.run([HIPCC] + build.HIPCC_FLAGS + ["--cuda-device-only", "-S", str(tmp_path / (element + ".hip")), "-o", str(tmp_path / (element + ".s"))],
+                       check=True, capture_output=True)
+        text = (tmp_path / (element + ".s")).read_text()
+        return text[text.index("amdhsa.kernels:"):].split("  - .agpr_count:")[1:]
+
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        entries = sum(pool.map(compiled, ("false", "true")), [])
+    assert len(entries) == 2 * (len(attend) + 4)
+    for entry in entries:
+        name = re.search(r"\.name: +(\S+)", entry).group(1)
+        scratch = int(re.search(r"\.private_segment_fixed_size: +(\d+)", entry).group(1))
+        # (kListed is 1)
+        may = re.search(r"cached_attention_kernelILi128ELb[01]ELi1ELi[14]ELNS0_4RowsE1E", name) is not None
+        assert scratch <= (16 if may else 0), (name, scratch)
