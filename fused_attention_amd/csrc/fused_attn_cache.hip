@@ -144,8 +144,9 @@ struct AttendPlan {
 
 constexpr int64_t kMostSplits = 64;    // the join gives each a lane
 
-// A launch and what it takes, in microseconds as measured: `wgs` workgroups of the narrow or the wide kernel for a causal call
-// (what the caller asks for is not known where the workspace is sized, and the longest rows take the same).
+// In how many parts a launch cuts its keys and what it takes, in microseconds as measured, for a causal call (what the caller asks for
+// is not known where the workspace is sized, and the longest rows take the same).  The lengths are in device memory: every
+// estimate takes the page table to be as wide as the longest sequence, and is off where it is wider.
 struct Estimate {
     int64_t splits;
     float us;
@@ -159,8 +160,9 @@ float join_us(const View& p, int64_t splits, int64_t H) {
 // In how many parts the keys of `base` row tiles are cut, few rows.  On 14 shapes (up to 64 sequences, 256 to 131072 tokens)
 // against every other count of parts, the best one is chosen or one within 5 % of it: a wave takes 1 + H / 110 for a step of
 // 64 tokens, or what the bytes of all heads take at 4.8 TB/s where that is more, or the products of a compute unit's
-// workgroups, those beyond one per compute unit in whole rounds; and the second kernel 3.  (B16 Rkv12 H64, 1000 tokens: 9.9 us in one part, 12.8 in two; Rkv8 H128, 2000
-// tokens: 18.5 in one part, 12.4 in four, 11.4 in eight; 131072 tokens: 75.7 in 16, 58.5 in 32, 66.1 in 48, 60.7 in 64.)
+// workgroups, those beyond one per compute unit in whole rounds; and the second kernel 3.  (B16 Rkv12 H64, 1000 tokens: 9.9 us
+// in one part, 12.8 in two; Rkv8 H128, 2000 tokens: 18.5 in one part, 12.4 in four, 11.4 in eight; 131072 tokens: 75.7 in 16,
+// 58.5 in 32, 66.1 in 48, 60.7 in 64.)
 Estimate narrow_splits(const View& p, int64_t base, int64_t steps, int64_t H) {
     const float alone = 1.f + 0.009f * (float)H;
     const float bytes = 0.0273f * (float)H;              // a step of a workgroup's waves, by a 256th of the memory
@@ -180,30 +182,35 @@ Estimate narrow_splits(const View& p, int64_t base, int64_t steps, int64_t H) {
 
 // Many rows, the narrow kernel in one part: rounds of the workgroups that a chip holds, and what the products and exponentials
 // take in all; or the longest workgroup; or the codes, which every row tile reads, where they are more than the second-level caches
-// hold (8 tokens of 64 sequences of 1000, 40 heads on 8 of 128: 58 us, 55).  (fp16, causal, estimated and measured: 8 sequences of 1000 tokens of 12 heads of 64: 46, 51 us; 2000 rows
-// of each of 8 heads of 128 over 8000 tokens: 94, 99; 4096 tokens of 32 heads of 128: 251, 247.)
+// hold.  (Causal, estimated and measured: 8 sequences of 1000 tokens of 12 heads of 64: 46, 51 us; 2000 rows of each of 8
+// heads of 128 over 8000 tokens: 94, 99; 4096 tokens of 32 heads of 128: 251, 247; by the codes, 8 tokens of 64 sequences of 1000, 40
+// heads on 8 of 128: 58, 55.)
 float narrow_us(const View& p, int64_t base, float keys, int64_t steps, int64_t H) {
     const int64_t resident = H > 64 ? 2 * kNumCu : 3 * kNumCu;
     const float rate = H > 64 ? 1.5e6f : H > 32 ? 2.4e6f : 3.e6f;       // rows times keys; the rows of whole tiles
     const float whole = (H > 64 ? 9.f : 6.5f) * (float)ceil_div(base, resident) + (float)base * 32.f * keys / rate;
     const float longest = 6.f + (1.f + 0.009f * (float)H) * (float)ceil_div(steps, fa::cache::kAttendWaves);
     const float us = whole > longest ? whole : longest;
-    const float bytes = (float)p.B * (float)p.Rkv * keys * 2.f * (float)H, read = 6.f + (float)base / ((float)p.B * (float)p.Rkv) * bytes / 5.e6f;
+    const float heads = (float)p.B * (float)p.Rkv, bytes = heads * keys * 2.f * (float)H;
+    const float read = 6.f + (float)base / heads * bytes / 5.e6f;
     return bytes > 3.2e7f && read > us ? read : us;
 }
 
 // The wide kernel: the longest workgroup's tiles of 64 keys, or what the chip's workgroups take in all, of which a compute
 // unit holds one at head_dim 128 and two below; with one block of 16 rows a wave instead of two, two and three.  Then a tile
 // takes 0.6 of the time and there are twice as many workgroups: for calls that the longest workgroup bounds.  (The same three,
-// measured with two blocks and with one: 38, 33 us; 90, 91, each in four parts; 178, 199.  32 heads on 8 of 128: 1500 tokens 57, 43, by
-// the other kernel 59; 2048 behind 14336 515, 528.  8 tokens of 64 sequences of 1000, 40 heads on 8 of 128: 66, 33, by the other 55.)
+// measured with two blocks and with one: 38, 33 us; 90, 91, each in four parts; 178, 199.  32 heads on 8 of 128: 1500 tokens 57,
+// 43, by the other kernel 59; 2048 behind 14336 515, 528.  8 tokens of 64 sequences of 1000, 40 heads on 8 of 128: 66, 33, by the
+// other 55.)
 Estimate wide_us(const View& p, int64_t nq, int64_t most_keys, float keys, int64_t H) {
     Estimate best{1, 3.0e38f};
     const int64_t base = (int64_t)p.B * p.Rkv * ceil_div((int64_t)p.L * p.group, fa::cache::kWideWaves * 16 * nq);
     for (int64_t s = 1; s <= kMostSplits && (s == 1 || (base * s <= 4 * kNumCu && s * fa::cache::kWideKeys < most_keys)); ++s) {
         const float per_cu = (float)(base * s) / kNumCu;
         const float two = H > 64 ? 2.02f : (per_cu > 1.f ? 2.3f : 1.6f) - (H > 32 ? 0.f : 0.3f);
-        const float one = H > 64 ? 1.36f + (per_cu > 1.f ? 0.4f * ((per_cu < 2.f ? per_cu : 2.f) - 1.f) : 0.f) : H > 32 ? (per_cu > 1.f ? 1.65f : 1.17f) : (per_cu > 1.f ? 1.2f : 0.95f);
+        const float one = H > 64   ? 1.36f + (per_cu > 1.f ? 0.4f * ((per_cu < 2.f ? per_cu : 2.f) - 1.f) : 0.f)
+                          : H > 32 ? (per_cu > 1.f ? 1.65f : 1.17f)
+                                   : (per_cu > 1.f ? 1.2f : 0.95f);
         const float tile = nq == 2 ? two : one;
         const float all = nq == 1 ? (H > 64 ? 1.12f : 0.75f) * per_cu : H > 64 ? tile * (float)ceil_div(base * s, kNumCu) : 1.3f * per_cu;
         const float longest = tile * (float)ceil_div(most_keys, s * fa::cache::kWideKeys), whole = all * keys / (float)(s * fa::cache::kWideKeys);
