@@ -283,10 +283,13 @@ int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t
  * q and out as in fa_fwd_strided, fp16 or bfloat16 (FA_FLAG_BF16), whatever type the cache was filled from.
  * Accuracy: codes enter both products as they are; scores, sums and outputs are float32; softmax weights are rounded to the
  * type of q.  fp16 weights keep 11 bits down to 2^-21 of the row's largest, and values 4 bits down to 2^-15 of the largest
- * power of two among the pages that a wave reads.
+ * power of two among the pages that a wave reads: pages without weight in the row are among them, and those that only
+ * rows beside it see.  With bfloat16 such a page costs no more than 2^-117 of its power of two.  scale * log2(e) times a page's power of
+ * two has to stay finite in float32.
  * A value that is not a number reaches the rows that see it only.
  * workspace: fa_cached_attention_workspace bytes of device memory, 16-byte aligned (FA_ERR_WORKSPACE if it is too small;
  * nullable where that is 0), not used by another call at the same time; nothing in it is kept between calls.
+ * The launch is chosen from the sizes: for sequences about as long as table_width allows.  Much wider tables cost time, not results.
  */
 int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,
                         void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, void* lse,
