@@ -760,6 +760,35 @@ def test_attention_over_pages_of_different_sizes(gpu, dtype, H, R, L, kernel):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,R,L,kernel", [(64, 4, 1, "few"), (64, 4, 9, "few"), (64, 256, 90, "many"), (128, 128, 90, "many")])
+@pytest.mark.parametrize("dtype,large,small", [(torch.float16, 0, -14), (torch.float16, 5, -20), (torch.bfloat16, 30, -80), (torch.bfloat16, 60, -80)])
+def test_small_values_beside_large_ones_without_weight(gpu, dtype, large, small, H, R, L, kernel):
+    # A page of large values that every row sees and gives no weight to: what the header says of the others' bits.  The tolerance is that of
+    # the attention without the large page, and of a value next to its power of two: half a step of the smallest fp16 numbers,
+    # 2^-25, or with bfloat16 the largest code, below 2^9, times the least scale of its conversion, 2^-126.
+    p = Problem(B=2, L=L, R=R, Rkv=2, H=H, P=16, W=10, dtype=dtype, seed=25)
+    assert capi.cached_attention_plan(2, L, R, 2, H, 16, 10)["kernel"] == kernel
+    p.starts = [160 - L, 70]
+    p.q[:] = p.q[:1, :1, :1].clone()                               # every row the same, and a key far below all others: e^-100 at least
+    p.v_exponents[:] = small
+    at = p.page_table[:, 2].long()
+    p.v_exponents[at], p.k_exponents[at] = large, -3
+    p.k_cache[at] = (-448 * torch.sign(p.q[0, 0, 0].float())).expand(2, 2, 16, H).to(E4M3)
+    assert p.q[0, 0, 0].float().abs().sum() * 448 * 2.0 ** -3 / math.sqrt(H) > 100 + 4 * 448 * 2.0 ** -7
+    with_it = pc.attention(p.cache(), p.q, p.starts, p.lens)[0]
+    table, p.page_table[:, 2] = p.page_table.clone(), -1
+    want, _, spread, size = pc.attention(p.cache(), p.q, p.starts, p.lens)
+    p.page_table = table
+    assert ((with_it - want).abs() <= 2.0 ** -30 * spread).all()
+    u, least = (2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -8, 2.0 ** -117)
+    d = (H + 8) * 2.0 ** -24 * size + 20 * 2.0 ** -22              # no score beyond 20 in float32's exponential
+    tol = spread * (u + 2 * d[..., None] + 2.0 ** -21 + 2 * (160 + 64) * 2.0 ** -24) + u * want.abs() + 2.0 ** large * least
+    tol = tol + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    got = p.by_token(_attend(_entries(), p, p.on(gpu)), R).double()
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,R,L,kernel", [(64, 4, 9, "few"), (64, 256, 90, "many"), (128, 128, 90, "many")])
 def test_scores_too_small_for_a_factor(gpu, H, R, L, kernel):
     # the caller's scale times a page's power of two below any float32: what a row does not see stays out of it all the same
