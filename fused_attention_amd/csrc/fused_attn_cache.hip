@@ -384,7 +384,8 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     if (selected != nullptr && count < 1) return FA_ERR_BAD_SHAPE;
     if (selected == nullptr) count = 0;
     if ((rc = check_count(count)) != FA_OK) return rc;
-    if (!(scale > 0.f) || scale > 3.0e38f) return FA_ERR_BAD_SCALE;
+    p.scale_log2e = scale * 1.4426950408889634f;
+    if (!(scale > 0.f) || !std::isfinite(p.scale_log2e)) return FA_ERR_BAD_SCALE;
     const int64_t B = cache->sequences, H = cache->head_dim;
     p.qs = {q_stride_b, q_stride_h, q_stride_l};
     p.os = {out_stride_b, out_stride_h, out_stride_l};
@@ -408,7 +409,6 @@ int fa_cached_attention(const fa_cache* cache, const void* q, int64_t q_stride_b
     p.by_splits = fa::divisor(a.splits);
     p.by_heads = fa::divisor(cache->heads);
     p.by_group = fa::divisor(p.group);
-    p.scale_log2e = scale * 1.4426950408889634f;
     int power;                                           // scale_log2e is at least 2^(power - 1)
     std::frexp(p.scale_log2e, &power);
     p.least_exponent = -125 - power;

@@ -284,8 +284,8 @@ int fa_cache_append(const fa_cache* cache, const void* k, const void* v, int64_t
  * Accuracy: codes enter both products as they are; scores, sums and outputs are float32; softmax weights are rounded to the
  * type of q.  fp16 weights keep 11 bits down to 2^-21 of the row's largest, and values 4 bits down to 2^-15 of the largest
  * power of two among the pages that a wave reads: pages without weight in the row are among them, and those that only
- * rows beside it see.  With bfloat16 such a page costs no more than 2^-117 of its power of two.  scale * log2(e) times a page's power of
- * two has to stay finite in float32.
+ * rows beside it see.  With bfloat16 such a page costs no more than 2^-117 of its power of two.  scale * log2(e) has to be finite in
+ * float32 (FA_ERR_BAD_SCALE), and times the power of two of a page's keys as well: scores of pages beyond that may become NaN.
  * A value that is not a number reaches the rows that see it only.
  * workspace: fa_cached_attention_workspace bytes of device memory, 16-byte aligned (FA_ERR_WORKSPACE if it is too small;
  * nullable where that is 0), not used by another call at the same time; nothing in it is kept between calls.

@@ -306,6 +306,21 @@ def test_the_library_refuses_what_its_header_says():
     assert "page_size" in capi.strerror(-9) and "workspace" in capi.strerror(-10)
 
 
+def test_scales_beyond_float32_in_units_of_log2_are_refused():
+    # the kernels' exponentials are of base 2: scale * log2(e) would be infinite, and a score of zero times it NaN
+    lib = capi.load_library()
+    ok = 0x1000                                                    # never dereferenced: without a workspace, nothing is launched
+    c = capi.Cache(keys=ok, values=ok, key_exponents=ok, value_exponents=ok, page_table=ok, pages=10, heads=2, page_size=64, head_dim=64,
+                   sequences=1, table_width=4096, table_stride=4096)
+
+    def attend(scale):
+        return lib.fa_cached_attention(ctypes.byref(c), ok, 256, 64, 256, ok, 256, 64, 256, None, None, 0, ok, None, 1, 4, scale, 0, None, 0, None)
+
+    largest = torch.finfo(torch.float32).max
+    assert [attend(s) for s in (largest, 2.9e38, largest / math.log2(math.e) * 1.001)] == [-8] * 3
+    assert [attend(s) for s in (largest / math.log2(math.e) * 0.999, 1.0, 1e-38)] == [-10] * 3
+
+
 def test_outputs_whose_rows_overlap_are_refused():
     # by zero strides, by strides that are too small, between any two dimensions; rows that lie apart are not: with nothing else wrong
     # those calls fail later, at the workspace that they lack
