@@ -18,7 +18,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libfused_attn_gfx950.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-LIB_SOURCES = ["fused_attn_capi.hip", "fused_attn_cache.hip"]
+LIB_SOURCES = ["fused_attn_capi.hip", "fused_attn_cache.hip", "fused_attn_rotary.hip", "fused_attn_pages.hip", "fused_attn_latent.hip"]
 SMOKE_PATH = os.path.join(PKG_DIR, "fa_test")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 

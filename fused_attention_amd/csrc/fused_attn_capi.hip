@@ -631,7 +631,7 @@ const char* fa_strerror(int status) {
     switch (status) {
         case FA_OK: return "success";
         case FA_ERR_NULL_POINTER: return "fa_fwd: q, k, v and out must be non-null device pointers (fa_cache: and all that is not nullable)";
-        case FA_ERR_BAD_HEAD_DIM: return "fa_fwd: head_dim must be 16, 32, 64 or 128";
+        case FA_ERR_BAD_HEAD_DIM: return "fa_fwd: head_dim must be 16, 32, 64 or 128 (fa_rotate: a multiple of 16; fa_latent_cache, fa_expanded: widths as listed there)";
         case FA_ERR_BAD_SHAPE:
             return "fa_fwd: B, R and L must be at least 1 (fa_qkv_proj: and the feature counts multiples of 64; fa_cache: and every size, R a multiple of heads)";
         case FA_ERR_BAD_STRIDE:

@@ -272,6 +272,7 @@ torch::Tensor qkv_projection(torch::Tensor hidden, torch::Tensor weight, std::op
 }
 
 #include "fused_attn_cache_binding.inc"
+#include "fused_attn_latent_binding.inc"
 
 }  // namespace
 
@@ -324,4 +325,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("layout") = "blf",
           "The `count` pages whose keys may score highest, for each new token and key head: int32 [batch, seq_len, key heads, "
           "count], ascending, -1 behind the last.");
+    bind_latent(m);
 }

@@ -1,0 +1,324 @@
+// C ABI of the latent attention (include/fused_attn.h): argument validation, the choice of launch and the launches.
+#include "host_checks.hpp"
+#include "latent_kernels.hpp"
+
+namespace {
+
+using namespace fa::latent;
+
+// f(std::integral_constant<int, C>, std::integral_constant<int, DR>, std::bool_constant<BF>)
+template <class F>
+hipError_t for_latent(int64_t C, int64_t DR, bool bf, F f) {
+    auto with = [&](auto c, auto d) { return bf ? f(c, d, std::true_type{}) : f(c, d, std::false_type{}); };
+    auto wide = [&](auto c) { return DR == 32 ? with(c, std::integral_constant<int, 32>{}) : with(c, std::integral_constant<int, 64>{}); };
+    return C == 128 ? wide(std::integral_constant<int, 128>{}) : C == 256 ? wide(std::integral_constant<int, 256>{}) : wide(std::integral_constant<int, 512>{});
+}
+
+int check_sizes(const fa_latent_cache* c, int64_t L, int64_t R, View* p) {
+    if (c == nullptr) return FA_ERR_NULL_POINTER;
+    if ((c->latent_dim != 128 && c->latent_dim != 256 && c->latent_dim != 512) || (c->rope_dim != 32 && c->rope_dim != 64)) return FA_ERR_BAD_HEAD_DIM;
+    int log2_p = 4;
+    while (log2_p < 7 && ((int64_t)1 << log2_p) < c->page_size) ++log2_p;
+    if (c->page_size != (int64_t)1 << log2_p) return FA_ERR_BAD_PAGE;
+    if (c->pages < 1 || c->sequences < 1 || c->table_width < 1 || L < 1 || R < 1) return FA_ERR_BAD_SHAPE;
+    if (c->table_stride < 0 || (c->table_stride < c->table_width && c->sequences > 1)) return FA_ERR_BAD_STRIDE;
+    if (c->pages > kMaxInt || R > kMaxInt || L > kMaxInt || c->sequences > kMaxInt || !below(c->table_width, c->page_size, kMaxInt) ||
+        !below(L, R, kMaxInt) || !below(L * R, c->sequences, kMaxInt) || !below(c->table_stride, c->sequences, kMaxElems))
+        return FA_ERR_TOO_LARGE;
+    p->latents = static_cast<uint16_t*>(c->latents);
+    p->table = c->page_table;
+    p->table_stride = c->table_stride;
+    p->B = (int)c->sequences;
+    p->L = (int)L;
+    p->R = (int)R;
+    p->W = (int)c->table_width;
+    p->pages = (int)c->pages;
+    p->log2_p = log2_p;
+    return FA_OK;
+}
+
+int check_tensors(const fa_latent_cache* c, const int32_t* starts, const int32_t* new_lens, View* p) {
+    if (starts == nullptr || c->page_table == nullptr || c->latents == nullptr) return FA_ERR_NULL_POINTER;
+    if (!aligned(starts, 4) || !aligned(new_lens, 4) || !aligned(c->page_table, 4) || !aligned(c->latents, 16)) return FA_ERR_MISALIGNED;
+    p->starts = starts;
+    p->new_lens = new_lens;
+    return FA_OK;
+}
+
+// A tensor of one row a token.
+int check_rows(const void* t, int64_t stride_b, int64_t stride_l, int64_t B, int64_t L, int64_t n) {
+    return check_strided(t, {stride_b, 0, stride_l}, B, 1, L, n);
+}
+
+// [B, L, heads, n] by strides of its own, where a head may stand next to the next one's token: stride_l need not reach over a row.
+int check_heads(const void* t, const Strides3& s, int64_t B, int64_t heads, int64_t L, int64_t n) {
+    if (t == nullptr) return FA_ERR_NULL_POINTER;
+    if (s.b < 0 || s.h < 0 || s.l < 0 || s.b % 8 != 0 || s.h % 8 != 0 || s.l % 8 != 0) return FA_ERR_BAD_STRIDE;
+    if (!aligned(t, 16)) return FA_ERR_MISALIGNED;
+    if ((s.l > 0 && !below(L, s.l, kMaxElems)) || (s.h > 0 && !below(heads, s.h, kMaxElems)) || (s.b > 0 && !below(B, s.b, kMaxElems)))
+        return FA_ERR_TOO_LARGE;
+    (void)n;
+    return FA_OK;
+}
+
+bool scale_of(float scale, float* scale_log2e) {
+    *scale_log2e = scale * 1.4426950408889634f;
+    return scale > 0.f && std::isfinite(*scale_log2e);
+}
+
+struct Plan {
+    int nq;
+    int64_t tiles, splits, wgs;
+};
+
+constexpr int64_t kMostParts = 128;      // of a row's keys
+
+Plan plan_latent(const View& p, int64_t C, int64_t DR) {
+    Plan a;
+    const int64_t rows = (int64_t)p.L * p.R, steps = ceil_div((int64_t)p.W << p.log2_p, kKeys);
+    a.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    a.tiles = ceil_div(rows, 16 * a.nq);
+    const int64_t base = p.B * a.tiles;
+    a.splits = 1;
+    while (a.splits < kMostParts && base * a.splits * 2 <= kNumCu && a.splits * 2 <= steps) a.splits *= 2;
+    a.wgs = base * a.splits;
+    (void)C, (void)DR;
+    return a;
+}
+
+Plan plan_expanded(int64_t B, int64_t L, int64_t R, int64_t K) {
+    Plan a;
+    a.nq = L <= 128 || B * R * ceil_div(L, 256) < kNumCu ? 1 : 2;
+    a.tiles = ceil_div(L, kExpandedWaves * 16 * a.nq);
+    a.splits = 1;
+    const int64_t base = B * R * a.tiles, steps = ceil_div(K, kKeys);
+    while (a.splits < kMostParts && base * a.splits * 2 <= kNumCu && a.splits * 4 <= steps) a.splits *= 2;
+    a.wgs = base * a.splits;
+    return a;
+}
+
+int64_t parts_bytes(int64_t rows, int64_t splits, int64_t C) { return splits > 1 ? rows * splits * (C + 1) * 4 : 0; }
+
+int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
+    if (need > 0 && (workspace == nullptr || bytes < need)) return FA_ERR_WORKSPACE;
+    return need > 0 && !aligned(workspace, 16) ? FA_ERR_MISALIGNED : FA_OK;
+}
+
+template <int C, bool BF, class P>
+hipError_t join(const P& p, hipStream_t s) {
+    JoinParams j;
+    j.part_o = p.part_o;
+    j.part_lse = p.part_lse;
+    j.out = p.out;
+    j.os = p.os;
+    j.lse = p.lse;
+    j.rows = (int64_t)p.B * p.L * p.R;
+    j.L = p.L;
+    j.R = p.R;
+    j.splits = p.splits;
+    j.by_heads = fa::divisor(p.R);
+    j.by_tokens = fa::divisor(p.L);
+    return launch(latent_join_kernel<C, BF>, ceil_div(j.rows, 4), 256, j, 0, s);
+}
+
+int check_expanded(const fa_expanded* x) {
+    if (x == nullptr) return FA_ERR_NULL_POINTER;
+    if ((x->key_dim != 64 && x->key_dim != 128) || x->value_dim != x->key_dim || (x->rope_dim != 32 && x->rope_dim != 64)) return FA_ERR_BAD_HEAD_DIM;
+    const int64_t B = x->sequences, L = x->tokens, R = x->heads, K = x->keys;
+    if (B < 1 || L < 1 || R < 1 || K < 1) return FA_ERR_BAD_SHAPE;
+    if (B > kMaxInt || L > kMaxInt || R > kMaxInt || K > kMaxInt || !below(L, R, kMaxInt) || !below(L * R, B, kMaxInt)) return FA_ERR_TOO_LARGE;
+    return FA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_latent_append(const fa_latent_cache* cache, const void* c, int64_t c_stride_b, int64_t c_stride_l, const void* k, int64_t k_stride_b,
+                     int64_t k_stride_l, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, void* q_out,
+                     int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, const int32_t* starts, const int32_t* new_lens, int64_t L,
+                     int64_t R, const float* rope_cos, const float* rope_sin, int64_t rope_rows, int flags, void* stream) {
+    if ((flags & ~(FA_FLAG_BF16 | FA_FLAG_INTERLEAVED)) != 0) return FA_ERR_BAD_FLAGS;
+    AppendParams p;
+    int rc = check_sizes(cache, L, q != nullptr || cache == nullptr ? R : 1, &p);
+    if (rc == FA_OK) rc = check_tensors(cache, starts, new_lens, &p);
+    if (rc != FA_OK) return rc;
+    const int64_t B = cache->sequences, C = cache->latent_dim, DR = cache->rope_dim;
+    if ((rc = check_rows(c, c_stride_b, c_stride_l, B, L, C)) != FA_OK) return rc;
+    if ((rc = check_rows(k, k_stride_b, k_stride_l, B, L, DR)) != FA_OK) return rc;
+    p.qs = {q_stride_b, q_stride_h, q_stride_l};
+    p.qo = {out_stride_b, out_stride_h, out_stride_l};
+    if ((q == nullptr) != (q_out == nullptr)) return FA_ERR_NULL_POINTER;
+    if (q != nullptr && (rc = check_heads(q, p.qs, B, R, L, DR)) != FA_OK) return rc;
+    if (q != nullptr && (rc = check_written(q_out, p.qo, B, R, L, DR)) != FA_OK) return rc;
+    if ((rope_cos == nullptr) != (rope_sin == nullptr)) return FA_ERR_NULL_POINTER;
+    if (rope_cos != nullptr && rope_rows < 1) return FA_ERR_BAD_SHAPE;
+    if (!aligned(rope_cos, 16) || !aligned(rope_sin, 16)) return FA_ERR_MISALIGNED;
+    if (!below(B * L, (C + DR) / 16, kMaxInt) || (q != nullptr && !below(B * L * R, DR / 16, kMaxInt))) return FA_ERR_TOO_LARGE;
+    p.c = static_cast<const uint16_t*>(c);
+    p.k = static_cast<const uint16_t*>(k);
+    p.c_stride_b = c_stride_b, p.c_stride_l = c_stride_l, p.k_stride_b = k_stride_b, p.k_stride_l = k_stride_l;
+    p.q = static_cast<const uint16_t*>(q);
+    p.q_out = static_cast<uint16_t*>(q_out);
+    p.cos = rope_cos;
+    p.sin = rope_sin;
+    p.rope_rows = rope_rows;
+    p.C = (int)C;
+    p.DR = (int)DR;
+    p.cache_units = B * L * ((C + DR) / 16);
+    p.q_units = q != nullptr ? B * L * R * (DR / 16) : 0;
+    p.by_units = fa::divisor((C + DR) / 16);
+    p.by_q_units = fa::divisor(DR / 16);
+    p.by_heads = fa::divisor(p.R);
+    p.by_tokens = fa::divisor(L);
+    const bool bf = (flags & FA_FLAG_BF16) != 0, il = (flags & FA_FLAG_INTERLEAVED) != 0;
+    auto kernel = bf ? (il ? latent_append_kernel<true, true> : latent_append_kernel<true, false>)
+                     : (il ? latent_append_kernel<false, true> : latent_append_kernel<false, false>);
+    return static_cast<int>(launch(kernel, ceil_div(p.cache_units + p.q_units, 256), 256, p, 0, static_cast<hipStream_t>(stream)));
+}
+
+int64_t fa_latent_attention_workspace(const fa_latent_cache* cache, int64_t L, int64_t R) {
+    View p;
+    const int rc = check_sizes(cache, L, R, &p);
+    if (rc != FA_OK) return rc;
+    return parts_bytes((int64_t)p.B * L * R, plan_latent(p, cache->latent_dim, cache->rope_dim).splits, cache->latent_dim);
+}
+
+int fa_latent_attention(const fa_latent_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, const void* r,
+                        int64_t r_stride_b, int64_t r_stride_h, int64_t r_stride_l, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                        int64_t out_stride_l, void* lse, const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R, float scale,
+                        int flags, void* workspace, int64_t workspace_bytes, void* stream) {
+    if ((flags & ~(FA_FLAG_BF16 | FA_FLAG_CAUSAL)) != 0) return FA_ERR_BAD_FLAGS;
+    AttendParams p;
+    int rc = check_sizes(cache, L, R, &p);
+    if (rc == FA_OK) rc = check_tensors(cache, starts, new_lens, &p);
+    if (rc != FA_OK) return rc;
+    if (!scale_of(scale, &p.scale_log2e)) return FA_ERR_BAD_SCALE;
+    const int64_t B = cache->sequences, C = cache->latent_dim, DR = cache->rope_dim;
+    p.qs = {q_stride_b, q_stride_h, q_stride_l};
+    p.rs = {r_stride_b, r_stride_h, r_stride_l};
+    p.os = {out_stride_b, out_stride_h, out_stride_l};
+    if ((rc = check_heads(q, p.qs, B, R, L, C)) != FA_OK) return rc;
+    if ((rc = check_heads(r, p.rs, B, R, L, DR)) != FA_OK) return rc;
+    if ((rc = check_written(out, p.os, B, R, L, C)) != FA_OK) return rc;
+    if (!aligned(lse, 4)) return FA_ERR_MISALIGNED;
+    const Plan a = plan_latent(p, C, DR);
+    if (a.wgs > kMaxInt || a.wgs > kMostThreads / 256) return FA_ERR_TOO_LARGE;
+    const int64_t rows = B * L * R;
+    if ((rc = check_workspace(workspace, workspace_bytes, parts_bytes(rows, a.splits, C))) != FA_OK) return rc;
+    p.q = static_cast<const uint16_t*>(q);
+    p.r = static_cast<const uint16_t*>(r);
+    p.out = static_cast<uint16_t*>(out);
+    p.lse = static_cast<float*>(lse);
+    p.causal = (flags & FA_FLAG_CAUSAL) != 0;
+    p.tiles = (int)a.tiles;
+    p.splits = (int)a.splits;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = p.part_o + rows * a.splits * C;
+    p.by_parts = fa::divisor(B * a.splits);
+    p.by_splits = fa::divisor(a.splits);
+    p.by_heads = fa::divisor(R);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return static_cast<int>(for_latent(C, DR, (flags & FA_FLAG_BF16) != 0, [&](auto c, auto d, auto bf) {
+        auto run = [&](auto nq) {
+            auto kernel = latent_attention_kernel<c(), d(), bf(), nq()>;
+            constexpr int lds = attend_lds_bytes<c(), d(), nq()>();
+            const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), lds);
+            return e != hipSuccess ? e : launch(kernel, a.wgs, 256, p, lds, s);
+        };
+        const hipError_t e = a.nq == 1   ? run(std::integral_constant<int, 1>{})
+                             : a.nq == 2 ? run(std::integral_constant<int, 2>{})
+                                         : run(std::integral_constant<int, 4>{});
+        return e != hipSuccess || a.splits == 1 ? e : join<c(), bf()>(p, s);
+    }));
+}
+
+int fa_latent_attention_plan(const fa_latent_cache* cache, int64_t L, int64_t R, int* plan) {
+    View p;
+    if (plan == nullptr) return FA_ERR_NULL_POINTER;
+    const int rc = check_sizes(cache, L, R, &p);
+    if (rc != FA_OK) return rc;
+    const Plan a = plan_latent(p, cache->latent_dim, cache->rope_dim);
+    if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
+    plan[0] = 16 * a.nq;
+    plan[1] = (int)a.splits;
+    plan[2] = (int)a.wgs;
+    return FA_OK;
+}
+
+int64_t fa_expanded_attention_workspace(const fa_expanded* x) {
+    const int rc = check_expanded(x);
+    if (rc != FA_OK) return rc;
+    return parts_bytes(x->sequences * x->tokens * x->heads, plan_expanded(x->sequences, x->tokens, x->heads, x->keys).splits, x->value_dim);
+}
+
+int fa_expanded_attention(const fa_expanded* x, float scale, int flags, void* workspace, int64_t workspace_bytes, void* stream) {
+    if ((flags & ~(FA_FLAG_BF16 | FA_FLAG_CAUSAL)) != 0) return FA_ERR_BAD_FLAGS;
+    int rc = check_expanded(x);
+    if (rc != FA_OK) return rc;
+    ExpandedParams p;
+    if (!scale_of(scale, &p.scale_log2e)) return FA_ERR_BAD_SCALE;
+    const int64_t B = x->sequences, L = x->tokens, R = x->heads, K = x->keys, D = x->key_dim, DR = x->rope_dim;
+    p.qs = {x->q_strides[0], x->q_strides[1], x->q_strides[2]};
+    p.ks = {x->k_strides[0], x->k_strides[1], x->k_strides[2]};
+    p.vs = {x->v_strides[0], x->v_strides[1], x->v_strides[2]};
+    p.os = {x->out_strides[0], x->out_strides[1], x->out_strides[2]};
+    p.kr_stride_b = x->rope_k_strides[0], p.kr_stride_l = x->rope_k_strides[1];
+    if ((rc = check_heads(x->q, p.qs, B, R, L, D + DR)) != FA_OK) return rc;
+    if ((rc = check_heads(x->k, p.ks, B, R, K, D)) != FA_OK) return rc;
+    if ((rc = check_heads(x->v, p.vs, B, R, K, D)) != FA_OK) return rc;
+    if ((rc = check_heads(x->rope_k, {p.kr_stride_b, 0, p.kr_stride_l}, B, 1, K, DR)) != FA_OK) return rc;
+    if ((rc = check_written(x->out, p.os, B, R, L, D)) != FA_OK) return rc;
+    if (!aligned(x->lse, 4) || !aligned(x->starts, 4) || !aligned(x->new_lens, 4)) return FA_ERR_MISALIGNED;
+    constexpr int64_t kMostStride = (int64_t)1 << 24;    // the loads' offsets within 16 keys have 32 bits
+    if (p.ks.l > kMostStride || p.vs.l > kMostStride || p.kr_stride_l > kMostStride) return FA_ERR_TOO_LARGE;
+    const Plan a = plan_expanded(B, L, R, K);
+    if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * kExpandedWaves)) return FA_ERR_TOO_LARGE;
+    const int64_t rows = B * L * R;
+    if ((rc = check_workspace(workspace, workspace_bytes, parts_bytes(rows, a.splits, D))) != FA_OK) return rc;
+    p.q = static_cast<const uint16_t*>(x->q);
+    p.k = static_cast<const uint16_t*>(x->k);
+    p.kr = static_cast<const uint16_t*>(x->rope_k);
+    p.v = static_cast<const uint16_t*>(x->v);
+    p.out = static_cast<uint16_t*>(x->out);
+    p.lse = static_cast<float*>(x->lse);
+    p.starts = x->starts;
+    p.new_lens = x->new_lens;
+    p.B = (int)B, p.L = (int)L, p.R = (int)R, p.K = (int)K;
+    p.causal = (flags & FA_FLAG_CAUSAL) != 0;
+    p.tiles = (int)a.tiles;
+    p.splits = (int)a.splits;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = p.part_o + rows * a.splits * D;
+    p.by_parts = fa::divisor(B * R * a.splits);
+    p.by_splits = fa::divisor(a.splits);
+    p.by_heads = fa::divisor(R);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto with = [&](auto d, auto dr, auto bf) {
+        auto run = [&](auto nq) {
+            auto kernel = expanded_attention_kernel<d(), dr(), bf(), nq()>;
+            constexpr int lds = Expanded<d(), dr()>::kLds;
+            const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), lds);
+            return e != hipSuccess ? e : launch(kernel, a.wgs, 64 * kExpandedWaves, p, lds, s);
+        };
+        const hipError_t e = a.nq == 1 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
+        return e != hipSuccess || a.splits == 1 ? e : join<d(), bf()>(p, s);
+    };
+    auto typed = [&](auto d, auto dr) { return (flags & FA_FLAG_BF16) != 0 ? with(d, dr, std::true_type{}) : with(d, dr, std::false_type{}); };
+    auto wide = [&](auto d) { return DR == 32 ? typed(d, std::integral_constant<int, 32>{}) : typed(d, std::integral_constant<int, 64>{}); };
+    return static_cast<int>(D == 64 ? wide(std::integral_constant<int, 64>{}) : wide(std::integral_constant<int, 128>{}));
+}
+
+int fa_expanded_attention_plan(const fa_expanded* x, int* plan) {
+    if (plan == nullptr) return FA_ERR_NULL_POINTER;
+    const int rc = check_expanded(x);
+    if (rc != FA_OK) return rc;
+    const Plan a = plan_expanded(x->sequences, x->tokens, x->heads, x->keys);
+    if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
+    plan[0] = 16 * a.nq * kExpandedWaves;
+    plan[1] = (int)a.splits;
+    plan[2] = (int)a.wgs;
+    return FA_OK;
+}
+
+}  // extern "C"

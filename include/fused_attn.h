@@ -39,6 +39,8 @@ extern "C" {
 
 #define FA_FLAG_CAUSAL 1
 #define FA_FLAG_BF16 2
+#define FA_FLAG_INTERLEAVED 4
+#define FA_FLAG_INVERSE 8
 
 /*
  * out = softmax(q k^T * scale [+ mask]) v for every (batch, head), non-causal.
@@ -325,6 +327,186 @@ int fa_select_pages(const fa_cache* cache, const void* q, int64_t q_stride_b, in
  */
 int fa_cached_attention_plan(const fa_cache* cache, int64_t L, int64_t R, int64_t count, int* plan);
 int fa_select_pages_plan(const fa_cache* cache, int64_t L, int64_t R, int* plan);
+
+/*
+ * Tables of a rotary position encoding, scaled for contexts longer than a model was made for: float32 [rows, dims / 2],
+ *     cos[p, j] = amplitude * cos(p f'_j),   sin[p, j] = amplitude * sin(p f'_j),   f_j = base^(-2 j / dims)
+ * in 64 bits, rounded once.  No counterpart in the reference, whose queries and keys come as they are
+ * (reference src/fused_attn_extention.cu:15-22).  scaling:
+ *   FA_ROTARY_NONE    f' = f
+ *   FA_ROTARY_LINEAR  f' = f / factor
+ *   FA_ROTARY_BASE    f' = (base * factor^(dims / (dims - 2)))^(-2 j / dims)
+ *   FA_ROTARY_TURNS   f' = f * (g + (1 - g) / factor) with t = original_rows * f / (2 pi), the turns of the column over the original
+ *                     context, and g = (t - low) / (high - low) within [0, 1]
+ *   FA_ROTARY_INDEX   the same with g = 1 - (j - a) / max(b - a, 0.001) within [0, 1], where
+ *                     i(t) = dims * ln(original_rows / (2 pi t)) / (2 ln base), a = max(floor(i(high)), 0), b = min(ceil(i(low)), dims - 1)
+ * base > 1; factor, original_rows, low < high and amplitude positive, where they are looked at, all finite (FA_ERR_BAD_SCALE).  dims is a
+ * multiple of 16 (FA_ERR_BAD_SHAPE) of at most 256 (FA_ERR_TOO_LARGE).  cos and sin 16-byte aligned.
+ */
+#define FA_ROTARY_NONE 0
+#define FA_ROTARY_LINEAR 1
+#define FA_ROTARY_BASE 2
+#define FA_ROTARY_TURNS 3
+#define FA_ROTARY_INDEX 4
+typedef struct fa_rotary {
+    int scaling;
+    double base, factor, original_rows, low, high, amplitude;
+} fa_rotary;
+
+int fa_rotary_tables(float* cos, float* sin, int64_t rows, int64_t dims, const fa_rotary* how, void* stream);
+
+/*
+ * Rotates queries, and keys (nullable, with k_out) beside them, by the positions of their tokens.  q has R heads and k has Rkv, of H
+ * channels (a multiple of 16 up to 1024), each with strides of its own under the addressing rule above, as have q_out and k_out.  The
+ * channels first .. first + dims of a head are rotated, the others copied; dims a multiple of 16, first of 8.  Pairs are the channels
+ * first + j and first + dims / 2 + j, or first + 2 j and first + 2 j + 1 with FA_FLAG_INTERLEAVED (j < dims / 2):
+ *     (a, b) -> (a cos - b sin, b cos + a sin)     with -sin for sin under FA_FLAG_INVERSE, which is also what a gradient needs
+ * each product and each sum rounded to float32, the result to 16 bits.  cos / sin: float32 [rope_rows, dims / 2], 16-byte aligned.
+ * Token i of sequence b has the position positions[b, i] (int32 [B, L], nullable) or starts[b] + i (int32 [B], nullable: zeros; not both:
+ * FA_ERR_BAD_SHAPE).  Rows of tokens behind new_lens[b] (int32 [B], nullable), or whose position is outside [0, rope_rows), become
+ * zeros.  out may be its input with the same strides; otherwise the two must not overlap.
+ */
+int fa_rotate(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, void* q_out, int64_t q_out_stride_b,
+              int64_t q_out_stride_h, int64_t q_out_stride_l, const void* k, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_l,
+              void* k_out, int64_t k_out_stride_b, int64_t k_out_stride_h, int64_t k_out_stride_l, int64_t B, int64_t L, int64_t R,
+              int64_t Rkv, int64_t H, int64_t first, int64_t dims, const float* cos, const float* sin, int64_t rope_rows,
+              const int32_t* positions, const int32_t* starts, const int32_t* new_lens, int flags, void* stream);
+
+/*
+ * Keeping the pages of a cache, the 8-bit one above or the one of latents below: all in device memory, so that a step never waits for
+ * the host.  No counterpart in the reference, which has no cache.
+ *
+ *   page_table  int32 [sequences, table_width], rows table_stride elements apart; a number outside [0, pages) is no page
+ *   starts      int32 [sequences]: tokens in the cache (not looked at by fa_copy_pages and fa_compact_pages)
+ *   uses        int32 [pages]: how many entries of the table name the page; a page without uses is free
+ *   data        `tensors` (up to 8) tensors of `pages` pages of page_bytes each, one behind the other: what a page holds
+ *               (looked at by fa_copy_pages, fa_fork_pages and fa_compact_pages)
+ *
+ * Lists are int32 in device memory; numbers in them that are no sequence, or no page, are passed over.  A count of 0 does nothing.
+ * Of a page's bytes 16 are moved at a time where the tensor is aligned to 16 and page_bytes is a multiple of it; otherwise 4, or 1.
+ */
+typedef struct fa_pages {
+    int32_t* page_table;
+    int32_t* starts;
+    int32_t* uses;
+    int64_t pages, page_size, sequences, table_width, table_stride;
+    int64_t tensors;
+    void* data[8];
+    int64_t page_bytes[8];
+} fa_pages;
+
+/* Page sources[n] into page targets[n] in all tensors, n < count.  A target is named once and is no source of another pair: what it
+ * holds otherwise is any mixture of the sources. */
+int fa_copy_pages(const fa_pages* pages, const int32_t* sources, const int32_t* targets, int64_t count, void* stream);
+
+/* The listed sequences end: every page of their rows loses a use, the rows become -1 and their starts 0.  Up to 65536 of them; one that
+ * is named twice ends once. */
+int fa_free_pages(const fa_pages* pages, const int32_t* sequences, int64_t count, void* stream);
+
+/*
+ * Pages for new tokens: sequence b brings new_lens[b] of them (nullable: L; within [0, L]), behind starts[b].  The places
+ * ceil(starts[b] / page_size) .. ceil((starts[b] + new_lens[b]) / page_size) of its row that name no page get the lowest free ones, in the
+ * order of the rows and places, and a use each.  missing, int32 [sequences], receives how many places found no page or lie behind
+ * the table; starts are left to the caller.  workspace: fa_take_pages_workspace bytes, 16-byte aligned, of no other call at the same time.
+ */
+int fa_take_pages(const fa_pages* pages, const int32_t* new_lens, int64_t L, int32_t* missing, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+int64_t fa_take_pages_workspace(const fa_pages* pages);
+
+/*
+ * Sequence children[n] continues sequence parents[n]: its row names the parent's full pages, which gain a use each, and where the
+ * parent's last page is not full the child gets a copy of it in the lowest free page (those of smaller n first).  Its starts
+ * become the parent's.  forked, int32 [count], receives 1; 0, and nothing else happens, where one of the two is no sequence, both are the same,
+ * the child has tokens, smaller n name the child as well, or no page is free for the copy.  All parents are as before the call.  Pages that
+ * an empty child's row names lose a use.  count is at most 4096 (FA_ERR_TOO_LARGE).  workspace as above.
+ */
+int fa_fork_pages(const fa_pages* pages, const int32_t* parents, const int32_t* children, int64_t count, int32_t* forked, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+int64_t fa_fork_pages_workspace(int64_t count);
+
+/*
+ * Moves the used pages together: of U used pages, those at U and above move, in ascending order, to the free places below U in
+ * ascending order, with their uses, and the table follows (entries that name a free page become -1).  moved, int32 [pages], receives
+ * where each used page is now, and -1 for the others.  workspace as above.
+ */
+int fa_compact_pages(const fa_pages* pages, int32_t* moved, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t fa_compact_pages_workspace(const fa_pages* pages);
+
+/*
+ * A paged cache of latents: for each token one vector of latent_dim channels that all heads share as key and as value, and one rotary
+ * key of rope_dim channels, latents [pages, page_size, latent_dim + rope_dim], contiguous, 16-byte aligned, fp16 or bfloat16
+ * (FA_FLAG_BF16).  page_table as in fa_cache.  latent_dim 128, 256 or 512, rope_dim 32 or 64 (FA_ERR_BAD_HEAD_DIM); page_size 16, 32, 64 or
+ * 128.  L, starts and new_lens as with fa_cache; positions are below table_width * page_size.  No counterpart in the reference.
+ */
+typedef struct fa_latent_cache {
+    void* latents;
+    const int32_t* page_table;
+    int64_t pages, page_size, latent_dim, rope_dim;
+    int64_t sequences, table_width, table_stride;
+} fa_latent_cache;
+
+/*
+ * Appends L new tokens per sequence: latents c [sequences, L, latent_dim] as they are, rotary keys k [sequences, L, rope_dim] rotated by
+ * their positions as fa_rotate does (tables [rope_rows, rope_dim / 2], both or neither; FA_FLAG_INTERLEAVED).  q (nullable: the rotary
+ * channels of R query heads, [sequences, L, R, rope_dim] by q_stride_b, _h, _l) is rotated likewise into q_out; rows of tokens that do not
+ * exist, or from rope_rows on, become zeros.  Nothing else of the cache is written.  A page that a call writes must belong to one sequence and
+ * stand once in its table.  c, k, q and q_out have 16-byte aligned addresses and strides that are multiples of 8 elements.
+ */
+int fa_latent_append(const fa_latent_cache* cache, const void* c, int64_t c_stride_b, int64_t c_stride_l, const void* k, int64_t k_stride_b,
+                     int64_t k_stride_l, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, void* q_out,
+                     int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_l, const int32_t* starts, const int32_t* new_lens, int64_t L,
+                     int64_t R, const float* rope_cos, const float* rope_sin, int64_t rope_rows, int flags, void* stream);
+
+/*
+ * Attention in the absorbed form: for each token and query head, with its queries q (latent_dim, the head's map of latents to keys
+ * multiplied in) and r (rope_dim, rotated),
+ *     s_j = scale * (q . c_j + r . k_j),   out = sum_j softmax(s)_j c_j   (latent_dim; the head's map to values is the caller's)
+ * over the cached tokens that fa_cached_attention would see: starts[b] + i + 1 with FA_FLAG_CAUSAL, otherwise starts[b] + new_lens[b], of
+ * those on a page.  q, r and out [sequences, L, R, .] by strides of their own.  Rows that see nothing, and those of tokens that do not
+ * exist, are zeros with an lse of -inf.  lse (nullable): float32 [sequences, R, L].  Scores, sums and outputs are float32; weights are rounded to the cache's type once.
+ * fp16 weights keep 11 bits down to 2^-22 of the row's largest and lose what is below 2^-32.  A latent or rotary key that is not finite makes rows
+ * that see it NaN where the formula does, or wholly; others never meet it.
+ * workspace: fa_latent_attention_workspace bytes, 16-byte aligned, of no other call at the same time (nullable where that is 0).  The launch is
+ * chosen from the sizes: for sequences about as long as table_width allows.
+ */
+int fa_latent_attention(const fa_latent_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, const void* r,
+                        int64_t r_stride_b, int64_t r_stride_h, int64_t r_stride_l, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                        int64_t out_stride_l, void* lse, const int32_t* starts, const int32_t* new_lens, int64_t L, int64_t R, float scale,
+                        int flags, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t fa_latent_attention_workspace(const fa_latent_cache* cache, int64_t L, int64_t R);
+
+/*
+ * Attention in the expanded form, for prompts: every head h has keys k and values v of its own, and all heads share the rotary keys,
+ *     s_j = scale * (q[: key_dim] . k_hj + q[key_dim :] . rope_k_j),   out = sum_j softmax(s)_j v_hj
+ * q [sequences, tokens, heads, key_dim + rope_dim], k [sequences, keys, heads, key_dim], rope_k [sequences, keys, rope_dim], v [sequences, keys,
+ * heads, value_dim], out [sequences, tokens, heads, value_dim] by strides {b, h, l} (rope_k: {b, l}) in elements, multiples of 8, those of the
+ * keys' dimension at most 2^24; fp16 or bfloat16.  key_dim = value_dim is 64 or 128, rope_dim 32 or 64 (FA_ERR_BAD_HEAD_DIM).  Token i of sequence b
+ * sees the first starts[b] + i + 1 keys with FA_FLAG_CAUSAL and starts[b] + new_lens[b] otherwise, of those there are (starts, int32
+ * [sequences], nullable: keys - tokens; new_lens nullable: tokens).  Rows, lse, workspace and accuracy as with fa_latent_attention; a value that is not finite
+ * makes rows that see it NaN or infinite in its channel, others never meet it.
+ */
+typedef struct fa_expanded {
+    const void* q;
+    const void* k;
+    const void* rope_k;
+    const void* v;
+    void* out;
+    void* lse;
+    const int32_t* starts;
+    const int32_t* new_lens;
+    int64_t sequences, tokens, heads, keys, key_dim, rope_dim, value_dim;
+    int64_t q_strides[3], k_strides[3], rope_k_strides[2], v_strides[3], out_strides[3];
+} fa_expanded;
+
+int fa_expanded_attention(const fa_expanded* x, float scale, int flags, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t fa_expanded_attention_workspace(const fa_expanded* x);
+
+/*
+ * The launches of the two for these sizes, without making them (no GPU is touched, only sizes are looked at): plan[0..2] = query rows per
+ * workgroup; parts that a row's keys are cut into; workgroups.
+ */
+int fa_latent_attention_plan(const fa_latent_cache* cache, int64_t L, int64_t R, int* plan);
+int fa_expanded_attention_plan(const fa_expanded* x, int* plan);
 
 #ifdef __cplusplus
 }
