@@ -999,7 +999,7 @@ def latent_attention_plan(B, L, R, C, DR, P, W, pages=1):
     out = (ctypes.c_int * 3)()
     _check(load_library().fa_latent_attention_plan(ctypes.byref(LatentCache(pages=pages, page_size=P, latent_dim=C, rope_dim=DR, sequences=B, table_width=W,
                                                                             table_stride=W)), L, R, out))
-    return dict(zip(("rows", "splits", "workgroups"), out))
+    return dict(zip(("rows", "shared", "workgroups"), out))
 
 
 def expanded_attention_plan(B, L, R, K, D, DR):

@@ -66,35 +66,69 @@ bool scale_of(float scale, float* scale_log2e) {
     return scale > 0.f && std::isfinite(*scale_log2e);
 }
 
+// How latent_attention is launched.
+struct LatentPlan {
+    int nq;
+    int64_t tiles, units, groups, wgs;       // groups: 0, a workgroup a unit
+    int least_share;
+};
+
+constexpr int64_t kMostUnits = 1024;         // that every workgroup adds up the lengths of
+
+LatentPlan plan_latent(const View& p, int64_t C) {
+    LatentPlan a;
+    const int64_t rows = (int64_t)p.L * p.R, steps = ceil_div((int64_t)p.W << p.log2_p, kKeys);
+    a.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    a.tiles = ceil_div(rows, 16 * a.nq);
+    a.units = p.B * a.tiles;
+    const int64_t resident = (C == 128 ? 2 : 1) * kNumCu;
+    // shares of at least two tiles, and none where one workgroup is through with its unit before a second kernel would be
+    // (C = 128, 4 tiles: 5 us, shared out 10)
+    a.least_share = 2;
+    a.groups = 0;
+    if (a.units <= kMostUnits && a.units < 2 * resident && steps > 2 + 768 / C && below(steps, a.units, 0x3fffffff)) {
+        const int64_t shares = a.units * ceil_div(steps, a.least_share);         // more have nothing to do
+        a.groups = shares < resident ? shares : resident;
+    }
+    a.wgs = a.groups > 0 ? a.groups : a.units;
+    return a;
+}
+
+// The parts' sums, their log-sum-exps and the plan.
+int64_t latent_workspace(const LatentPlan& a, int64_t C) {
+    return a.groups > 0 ? ((a.groups + a.units) * 16 * a.nq * (C + 1) + a.units + 2) * 4 : 0;
+}
+
+// How expanded_attention is launched.
 struct Plan {
     int nq;
     int64_t tiles, splits, wgs;
 };
 
-constexpr int64_t kMostParts = 128;      // of a row's keys
+// Waves that join the parts of a row, about so many of them.
+int join_waves(int64_t parts) { return parts >= 32 ? 16 : parts >= 8 ? 4 : 1; }
 
-Plan plan_latent(const View& p, int64_t C, int64_t DR) {
-    Plan a;
-    const int64_t rows = (int64_t)p.L * p.R, steps = ceil_div((int64_t)p.W << p.log2_p, kKeys);
-    a.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    a.tiles = ceil_div(rows, 16 * a.nq);
-    const int64_t base = p.B * a.tiles;
-    a.splits = 1;
-    while (a.splits < kMostParts && base * a.splits * 2 <= kNumCu && a.splits * 2 <= steps) a.splits *= 2;
-    a.wgs = base * a.splits;
-    (void)C, (void)DR;
-    return a;
-}
+constexpr int64_t kMostParts = 128;          // of a row's keys
 
-Plan plan_expanded(int64_t B, int64_t L, int64_t R, int64_t K) {
-    Plan a;
-    a.nq = L <= 128 || B * R * ceil_div(L, 256) < kNumCu ? 1 : 2;
-    a.tiles = ceil_div(L, kExpandedWaves * 16 * a.nq);
-    a.splits = 1;
-    const int64_t base = B * R * a.tiles, steps = ceil_div(K, kKeys);
-    while (a.splits < kMostParts && base * a.splits * 2 <= kNumCu && a.splits * 4 <= steps) a.splits *= 2;
-    a.wgs = base * a.splits;
-    return a;
+// Rows of a workgroup and parts of the keys by what a launch is estimated to take, causal (what the caller asks for is not known where the
+// workspace is sized): the longest workgroup's tiles, each `alone` us, or all tiles by what a compute unit takes for one, and the second
+// kernel's.  (Measured, with 128 and with 256 rows, us: 8 sequences of 1001 tokens of 12 heads of 64: 36, 38; 4 of them 27, 33; 2048
+// tokens of 16 heads of 128, 4 sequences 142, 111; one of 4096 118, 152; 4096 behind 12288, 32 heads 1357, 1067.)
+Plan plan_expanded(int64_t B, int64_t L, int64_t R, int64_t K, int64_t D) {
+    Plan best = {};
+    float best_us = 3.0e38f;
+    const float longest = (float)ceil_div(K, kKeys), mean = K > L ? ((float)K - 0.5f * (float)L) / kKeys : 0.5f * longest;
+    for (int nq = 1; nq <= 2; ++nq) {
+        const float alone = D == 128 ? (nq == 2 ? 2.2f : 1.4f) : (nq == 2 ? 1.65f : 1.3f), each = D == 128 ? alone : (nq == 2 ? 1.65f : 0.9f);
+        const int64_t tiles = ceil_div(L, kExpandedWaves * 16 * nq), base = B * R * tiles;
+        for (int64_t s = 1; s <= kMostParts && (s == 1 || (base * s <= 4 * kNumCu && 2 * s <= ceil_div(K, kKeys))); s *= 2) {
+            const float chain = alone * (float)ceil_div((int64_t)longest, s), all = each * (float)base * (mean < longest ? mean : longest) / kNumCu;
+            const float join = s > 1 ? 4.f + (float)(B * L * R) * (float)(s * D) * 8.f / 2.5e6f : 0.f;
+            const float us = 6.f + (chain > all ? chain : all) + join;
+            if (us < best_us) best_us = us, best = {nq, tiles, s, base * s};
+        }
+    }
+    return best;
 }
 
 int64_t parts_bytes(int64_t rows, int64_t splits, int64_t C) { return splits > 1 ? rows * splits * (C + 1) * 4 : 0; }
@@ -102,23 +136,6 @@ int64_t parts_bytes(int64_t rows, int64_t splits, int64_t C) { return splits > 1
 int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
     if (need > 0 && (workspace == nullptr || bytes < need)) return FA_ERR_WORKSPACE;
     return need > 0 && !aligned(workspace, 16) ? FA_ERR_MISALIGNED : FA_OK;
-}
-
-template <int C, bool BF, class P>
-hipError_t join(const P& p, hipStream_t s) {
-    JoinParams j;
-    j.part_o = p.part_o;
-    j.part_lse = p.part_lse;
-    j.out = p.out;
-    j.os = p.os;
-    j.lse = p.lse;
-    j.rows = (int64_t)p.B * p.L * p.R;
-    j.L = p.L;
-    j.R = p.R;
-    j.splits = p.splits;
-    j.by_heads = fa::divisor(p.R);
-    j.by_tokens = fa::divisor(p.L);
-    return launch(latent_join_kernel<C, BF>, ceil_div(j.rows, 4), 256, j, 0, s);
 }
 
 int check_expanded(const fa_expanded* x) {
@@ -181,7 +198,7 @@ int64_t fa_latent_attention_workspace(const fa_latent_cache* cache, int64_t L, i
     View p;
     const int rc = check_sizes(cache, L, R, &p);
     if (rc != FA_OK) return rc;
-    return parts_bytes((int64_t)p.B * L * R, plan_latent(p, cache->latent_dim, cache->rope_dim).splits, cache->latent_dim);
+    return latent_workspace(plan_latent(p, cache->latent_dim), cache->latent_dim);
 }
 
 int fa_latent_attention(const fa_latent_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, const void* r,
@@ -202,34 +219,41 @@ int fa_latent_attention(const fa_latent_cache* cache, const void* q, int64_t q_s
     if ((rc = check_heads(r, p.rs, B, R, L, DR)) != FA_OK) return rc;
     if ((rc = check_written(out, p.os, B, R, L, C)) != FA_OK) return rc;
     if (!aligned(lse, 4)) return FA_ERR_MISALIGNED;
-    const Plan a = plan_latent(p, C, DR);
-    if (a.wgs > kMaxInt || a.wgs > kMostThreads / 256) return FA_ERR_TOO_LARGE;
-    const int64_t rows = B * L * R;
-    if ((rc = check_workspace(workspace, workspace_bytes, parts_bytes(rows, a.splits, C))) != FA_OK) return rc;
+    const LatentPlan a = plan_latent(p, C);
+    if (a.wgs > kMaxInt || a.wgs > kMostThreads / 512) return FA_ERR_TOO_LARGE;
+    if ((rc = check_workspace(workspace, workspace_bytes, latent_workspace(a, C))) != FA_OK) return rc;
     p.q = static_cast<const uint16_t*>(q);
     p.r = static_cast<const uint16_t*>(r);
     p.out = static_cast<uint16_t*>(out);
     p.lse = static_cast<float*>(lse);
     p.causal = (flags & FA_FLAG_CAUSAL) != 0;
     p.tiles = (int)a.tiles;
-    p.splits = (int)a.splits;
+    p.units = (int)a.units;
+    p.groups = (int)a.groups;
+    p.least_share = a.least_share;
+    p.rows_of_unit = 16 * a.nq;
+    const int64_t parts = (a.groups + a.units) * 16 * a.nq;
     p.part_o = static_cast<float*>(workspace);
-    p.part_lse = p.part_o + rows * a.splits * C;
-    p.by_parts = fa::divisor(B * a.splits);
-    p.by_splits = fa::divisor(a.splits);
+    p.part_lse = p.part_o + parts * C;
+    p.plan = reinterpret_cast<int32_t*>(p.part_lse + parts);
     p.by_heads = fa::divisor(R);
+    p.by_tiles = fa::divisor(a.tiles);
+    p.by_sequences = fa::divisor(B);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return static_cast<int>(for_latent(C, DR, (flags & FA_FLAG_BF16) != 0, [&](auto c, auto d, auto bf) {
         auto run = [&](auto nq) {
+            using S = Shape<c(), d(), nq()>;
             auto kernel = latent_attention_kernel<c(), d(), bf(), nq()>;
-            constexpr int lds = attend_lds_bytes<c(), d(), nq()>();
-            const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), lds);
-            return e != hipSuccess ? e : launch(kernel, a.wgs, 256, p, lds, s);
+            const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), S::kLds);
+            return e != hipSuccess ? e : launch(kernel, a.wgs, 64 * S::WAVES, p, S::kLds, s);
         };
         const hipError_t e = a.nq == 1   ? run(std::integral_constant<int, 1>{})
                              : a.nq == 2 ? run(std::integral_constant<int, 2>{})
                                          : run(std::integral_constant<int, 4>{});
-        return e != hipSuccess || a.splits == 1 ? e : join<c(), bf()>(p, s);
+        if (e != hipSuccess || a.groups == 0) return e;
+        const int waves = join_waves(a.groups / a.units);
+        auto kernel = waves == 16 ? latent_join_kernel<c(), bf(), 16> : waves == 4 ? latent_join_kernel<c(), bf(), 4> : latent_join_kernel<c(), bf(), 1>;
+        return launch(kernel, ceil_div(B * L * R, rows_of_join(waves)), waves > 1 ? 64 * waves : 256, p, 0, s);
     }));
 }
 
@@ -238,10 +262,10 @@ int fa_latent_attention_plan(const fa_latent_cache* cache, int64_t L, int64_t R,
     if (plan == nullptr) return FA_ERR_NULL_POINTER;
     const int rc = check_sizes(cache, L, R, &p);
     if (rc != FA_OK) return rc;
-    const Plan a = plan_latent(p, cache->latent_dim, cache->rope_dim);
+    const LatentPlan a = plan_latent(p, cache->latent_dim);
     if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
     plan[0] = 16 * a.nq;
-    plan[1] = (int)a.splits;
+    plan[1] = a.groups > 0;
     plan[2] = (int)a.wgs;
     return FA_OK;
 }
@@ -249,7 +273,7 @@ int fa_latent_attention_plan(const fa_latent_cache* cache, int64_t L, int64_t R,
 int64_t fa_expanded_attention_workspace(const fa_expanded* x) {
     const int rc = check_expanded(x);
     if (rc != FA_OK) return rc;
-    return parts_bytes(x->sequences * x->tokens * x->heads, plan_expanded(x->sequences, x->tokens, x->heads, x->keys).splits, x->value_dim);
+    return parts_bytes(x->sequences * x->tokens * x->heads, plan_expanded(x->sequences, x->tokens, x->heads, x->keys, x->key_dim).splits, x->value_dim);
 }
 
 int fa_expanded_attention(const fa_expanded* x, float scale, int flags, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -272,7 +296,7 @@ int fa_expanded_attention(const fa_expanded* x, float scale, int flags, void* wo
     if (!aligned(x->lse, 4) || !aligned(x->starts, 4) || !aligned(x->new_lens, 4)) return FA_ERR_MISALIGNED;
     constexpr int64_t kMostStride = (int64_t)1 << 24;    // the loads' offsets within 16 keys have 32 bits
     if (p.ks.l > kMostStride || p.vs.l > kMostStride || p.kr_stride_l > kMostStride) return FA_ERR_TOO_LARGE;
-    const Plan a = plan_expanded(B, L, R, K);
+    const Plan a = plan_expanded(B, L, R, K, D);
     if (a.wgs > kMaxInt || a.wgs > kMostThreads / (64 * kExpandedWaves)) return FA_ERR_TOO_LARGE;
     const int64_t rows = B * L * R;
     if ((rc = check_workspace(workspace, workspace_bytes, parts_bytes(rows, a.splits, D))) != FA_OK) return rc;
@@ -302,7 +326,10 @@ int fa_expanded_attention(const fa_expanded* x, float scale, int flags, void* wo
             return e != hipSuccess ? e : launch(kernel, a.wgs, 64 * kExpandedWaves, p, lds, s);
         };
         const hipError_t e = a.nq == 1 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
-        return e != hipSuccess || a.splits == 1 ? e : join<d(), bf()>(p, s);
+        if (e != hipSuccess || a.splits == 1) return e;
+        const int waves = join_waves(a.splits);
+        auto kernel = waves == 16 ? expanded_join_kernel<d(), bf(), 16> : waves == 4 ? expanded_join_kernel<d(), bf(), 4> : expanded_join_kernel<d(), bf(), 1>;
+        return launch(kernel, ceil_div(rows, rows_of_join(waves)), waves > 1 ? 64 * waves : 256, p, 0, s);
     };
     auto typed = [&](auto d, auto dr) { return (flags & FA_FLAG_BF16) != 0 ? with(d, dr, std::true_type{}) : with(d, dr, std::false_type{}); };
     auto wide = [&](auto d) { return DR == 32 ? typed(d, std::integral_constant<int, 32>{}) : typed(d, std::integral_constant<int, 64>{}); };
@@ -313,7 +340,7 @@ int fa_expanded_attention_plan(const fa_expanded* x, int* plan) {
     if (plan == nullptr) return FA_ERR_NULL_POINTER;
     const int rc = check_expanded(x);
     if (rc != FA_OK) return rc;
-    const Plan a = plan_expanded(x->sequences, x->tokens, x->heads, x->keys);
+    const Plan a = plan_expanded(x->sequences, x->tokens, x->heads, x->keys, x->key_dim);
     if (a.wgs > kMaxInt) return FA_ERR_TOO_LARGE;
     plan[0] = 16 * a.nq * kExpandedWaves;
     plan[1] = (int)a.splits;

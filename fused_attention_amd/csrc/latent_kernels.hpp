@@ -12,8 +12,9 @@
 //
 // LDS holds keys and values as blocks of 16 tokens by 32 channels, 1 KiB, written by one direct-to-LDS load of a wave: lane l brings 16
 // bytes of token l / 4, so that four lanes read 64 bytes in a row and the lane's offset is the same for every block.  Which of the four
-// quarters lane l brings is (l % 4) ^ (l / 16): the 16 lanes that read one quarter of 16 tokens as an operand, and the 16 that read
-// four tokens by 16 channels for a transpose, then touch all banks alike.
+// quarters lane l brings is (l % 4) ^ quarter_of(l / 16), so that the lanes that LDS serves at once, lanes 0..3, 12..15, 20..23 and 24..27
+// of a 16-byte read and so on, and 32 lanes in a row of a transposing one, meet in no bank.  (With l / 16 in its place, as 16 lanes in a
+// row would have it, LDS lost half as many cycles again to conflicts as it worked.)
 #pragma once
 
 #include "rotation.hpp"
@@ -128,23 +129,36 @@ template <bool BF>
 constexpr float kBias = BF ? 0.f : 8.f;
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// A value that the compiler does not know to be the one it was: what follows from it is not worked out ahead of a loop and kept through it.
+__device__ __forceinline__ int afresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t afresh_uniform(uint32_t x) {
+    x = __builtin_amdgcn_readfirstlane(x);
+    asm volatile("" : "+s"(x));
+    return x;
+}
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// Of the tokens 4 k .. 4 k + 3 of a block: what their quarters' numbers are changed by.
+__device__ __forceinline__ int quarter_of(int k) { return (2 * k & 3) ^ (k & 2 ? 3 : 0); }     // 0, 2, 3, 1
+
 // Lane's bytes within a block: as loaded from rows `row_bytes` apart, as an operand of the first product, and as a transposed one of
 // the second (channel tiles with an even and an odd number).
 __device__ __forceinline__ uint32_t from_row(int lane, uint32_t row_bytes) {
-    return (uint32_t)(lane >> 2) * row_bytes + (uint32_t)((lane & 3) ^ (lane >> 4)) * 16u;
+    return (uint32_t)(lane >> 2) * row_bytes + (uint32_t)((lane & 3) ^ quarter_of(lane >> 4)) * 16u;
 }
 __device__ __forceinline__ int key_at(int lane) {
     const int c = lane & 15, g = lane >> 4;
-    return (4 * c + (g ^ (c >> 2))) * 16;
+    return (4 * c + (g ^ quarter_of(c >> 2))) * 16;
 }
 __device__ __forceinline__ int value_at(int lane, int odd) {
     const int s = lane & 15, g = lane >> 4;
-    return ((4 * g + (s >> 2)) * 4 + ((2 * odd + ((s & 3) >> 1)) ^ g)) * 16 + (s & 1) * 8;
+    return ((4 * g + (s >> 2)) * 4 + ((2 * odd + ((s & 3) >> 1)) ^ quarter_of(g))) * 16 + (s & 1) * 8;
 }
 
 __device__ __forceinline__ u32x2 read_transposed(const uint8_t* at) {
@@ -161,57 +175,70 @@ __device__ __forceinline__ bool not_finite(u32x4 x) {
     return (any & 0x80008000u) != 0;
 }
 
-// Joins the parts that a row's keys were cut into: a wave a row, C / 8 lanes with eight channels each, the parts dealt out to the
-// others and summed in a fixed order.  A part without any key has nothing but its log-sum-exp, -inf.
-struct JoinParams {
-    const float* part_o;       // [rows, splits, C]
-    const float* part_lse;     // [rows, splits], log2 units
-    uint16_t* out;
-    Strides3 os;
-    float* lse;                // [B, R, L] or nullptr
-    int64_t rows;
-    int L, R, splits;
-    Divisor by_heads, by_tokens;
-};
-template <int C, bool BF>
-__global__ __launch_bounds__(256) void latent_join_kernel(const JoinParams p) {
-    constexpr int kLanes = C / 8, kAtOnce = 64 / kLanes;
-    const int lane = threadIdx.x & 63, d = lane % kLanes * 8;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= p.rows) return;
-    const float* parts = p.part_lse + row * p.splits;
+// Joins the parts that a row's keys were cut into: WAVES waves a row, of each C / 8 lanes with eight channels, the parts dealt out to
+// waves and lane groups and summed in a fixed order.  A part without any key has nothing but its log-sum-exp, -inf.  `part_lse` and
+// `part_o`: the first part, the others `stride` rows further on each.
+template <int C, bool BF, int WAVES>
+__device__ __forceinline__ void join_row(const float* part_lse, const float* part_o, int parts, int64_t stride, uint16_t* out, float* lse) {
+    constexpr int kLanes = C / 8, kAtOnce = 64 / kLanes * WAVES;
+    __shared__ float exchange[WAVES > 1 ? WAVES : 1][C];
+    const int lane = threadIdx.x & 63, wave = WAVES > 1 ? threadIdx.x >> 6 : 0, d = lane % kLanes * 8;
     float top = -__builtin_inff();
-    for (int s = lane; s < p.splits; s += 64) top = fmax2(top, parts[s]);
+    for (int s = lane; s < parts; s += 64) top = fmax2(top, part_lse[s * stride]);
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) top = fmax2(top, __shfl_xor(top, s));
     const float less = top == -__builtin_inff() ? 0.f : top;
     float total = 0.f;
-    for (int s = lane; s < p.splits; s += 64) total += exp2_fast(parts[s] - less);
+    for (int s = lane; s < parts; s += 64) total += exp2_fast(part_lse[s * stride] - less);
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s);
     float y[8] = {};
-    for (int s = lane / kLanes; s < p.splits; s += kAtOnce) {
-        const float part = parts[s];
-        if (part == -__builtin_inff()) continue;
-        const float w = exp2_fast(part - less);
-        const floatx4* from = reinterpret_cast<const floatx4*>(p.part_o + (row * p.splits + s) * C + d);
+#pragma unroll 4
+    for (int s = wave * (64 / kLanes) + lane / kLanes; s < parts; s += kAtOnce) {
+        const float part = part_lse[s * stride], w = exp2_fast(part - less);
+        const floatx4* from = reinterpret_cast<const floatx4*>(part_o + s * stride * C + d);
         const floatx4 a = from[0], b = from[1];
+        const bool empty = part == -__builtin_inff();    // nothing was written there
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] += w * a[j], y[4 + j] += w * b[j];
+        for (int j = 0; j < 4; ++j) y[j] += empty ? 0.f : w * a[j], y[4 + j] += empty ? 0.f : w * b[j];
     }
 #pragma unroll
     for (int s = kLanes; s < 64; s <<= 1)
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] += __shfl_xor(y[j], s);
+    if constexpr (WAVES > 1) {
+        if (lane < kLanes) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) exchange[wave][d + j] = y[j];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] += exchange[w][d + j];
+    }
     if (lane >= kLanes) return;
     const float inv = total == 0.f ? 0.f : 1.f / total;
     u32x4 r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = Elem<BF>::pack(y[2 * j] * inv, y[2 * j + 1] * inv);
-    const int token = p.by_heads.of((int)row), head = (int)row - token * p.R, b = p.by_tokens.of(token), i = token - b * p.L;
-    *reinterpret_cast<u32x4*>(p.out + b * p.os.b + head * p.os.h + i * p.os.l + d) = r;
-    if (d == 0 && p.lse != nullptr)
-        p.lse[((int64_t)b * p.R + head) * p.L + i] = total == 0.f ? -__builtin_inff() : (less + __log2f(total)) * 0.6931471805599453f;
+    *reinterpret_cast<u32x4*>(out + d) = r;
+    if (d == 0 && lse != nullptr) *lse = total == 0.f ? -__builtin_inff() : (less + __log2f(total)) * 0.6931471805599453f;
+}
+// Rows of a workgroup of the joining kernels.
+constexpr int rows_of_join(int waves) { return waves > 1 ? 1 : 4; }
+
+// A direct-to-LDS load from an address of each lane's own.
+__device__ __forceinline__ void lds_load16(uint32_t lds_addr, const uint16_t* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_addr), "v"(from) : "memory", "m0");
+}
+
+// ... from addresses next to each other, by all lanes (lanes = ~0) or none (0).  Not said to change memory, so that reads of other rooms may pass it: those of
+// its own room stand behind a barrier, which does say so.
+__device__ __forceinline__ void masked_dma16(uint32_t lds_addr, const uint16_t* base, uint32_t voff, uint32_t lanes) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1" ::"s"(lds_addr), "v"(voff),
+                 "s"(base), "s"(lanes) : "m0");
 }
 
 #include "latent_attend.inc"

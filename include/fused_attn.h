@@ -503,7 +503,8 @@ int64_t fa_expanded_attention_workspace(const fa_expanded* x);
 
 /*
  * The launches of the two for these sizes, without making them (no GPU is touched, only sizes are looked at): plan[0..2] = query rows per
- * workgroup; parts that a row's keys are cut into; workgroups.
+ * workgroup; for fa_latent_attention 1 where the workgroups share out the keys of all rows and 0 where each has rows to itself, for
+ * fa_expanded_attention the parts that a row's keys are cut into; workgroups.
  */
 int fa_latent_attention_plan(const fa_latent_cache* cache, int64_t L, int64_t R, int* plan);
 int fa_expanded_attention_plan(const fa_expanded* x, int* plan);
