@@ -12,6 +12,7 @@ bool turns_of(const fa_rotary* r, int64_t dims, double* turns) {
     const double two_pi = 6.283185307179586476925;
     double base = r->base;
     if (r->scaling == FA_ROTARY_BASE) base *= std::pow(r->factor, (double)dims / (double)(dims - 2));
+    if (!std::isfinite(base)) return false;
     double low = 0, high = 0;
     if (r->scaling == FA_ROTARY_INDEX) {
         auto index = [&](double t) { return (double)dims * std::log(r->original_rows / (two_pi * t)) / (2 * std::log(base)); };
