@@ -73,30 +73,33 @@ struct LatentPlan {
     int least_share;
 };
 
-constexpr int64_t kMostUnits = 1024;         // that every workgroup adds up the lengths of
-
+// Rows of a workgroup by what a launch is estimated to take: tiles of 64 rows take less for each row, of 32 less to begin and to join.
+// (C = 512, us, 32 and 64 rows, with the joining: 16 sequences of 2000 tokens, 160 rows each 36, 38; 2 of them 22, 25; one of 32000
+// 35, 38; 128 rows of one of 131072 73, 65.)
 LatentPlan plan_latent(const View& p, int64_t C) {
     LatentPlan a;
-    const int64_t rows = (int64_t)p.L * p.R, steps = ceil_div((int64_t)p.W << p.log2_p, kKeys);
-    a.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const int64_t rows = (int64_t)p.L * p.R, steps = ceil_div((int64_t)p.W << p.log2_p, kKeys), resident = (C == 128 ? 2 : 1) * kNumCu;
+    a.least_share = 2;                       // key tiles
+    auto estimate = [&](int nq) {            // us / 0.4
+        const double units = (double)p.B * (double)ceil_div(rows, 16 * nq), shares = units * (double)ceil_div(steps, a.least_share);
+        return (nq == 2 ? 20. : 27.) + (nq == 2 ? 3.3 : 4.6) * units * (double)steps / (shares < (double)resident ? shares : (double)resident);
+    };
+    a.nq = rows <= 16 ? 1 : rows <= 32 || estimate(2) < estimate(4) ? 2 : 4;
     a.tiles = ceil_div(rows, 16 * a.nq);
     a.units = p.B * a.tiles;
-    const int64_t resident = (C == 128 ? 2 : 1) * kNumCu;
-    // shares of at least two tiles, and none where one workgroup is through with its unit before a second kernel would be
-    // (C = 128, 4 tiles: 5 us, shared out 10)
-    a.least_share = 2;
+    // None shared out where one workgroup is through with its unit before a second kernel would be (C = 128, 4 tiles: 5 us, shared out 10).
     a.groups = 0;
     if (a.units <= kMostUnits && a.units < 2 * resident && steps > 2 + 768 / C && below(steps, a.units, 0x3fffffff)) {
         const int64_t shares = a.units * ceil_div(steps, a.least_share);         // more have nothing to do
         a.groups = shares < resident ? shares : resident;
     }
-    a.wgs = a.groups > 0 ? a.groups : a.units;
+    a.wgs = a.groups > 0 ? ceil_div(a.groups, 8) * 8 : a.units;
     return a;
 }
 
 // The parts' sums, their log-sum-exps and the plan.
 int64_t latent_workspace(const LatentPlan& a, int64_t C) {
-    return a.groups > 0 ? ((a.groups + a.units) * 16 * a.nq * (C + 1) + a.units + 2) * 4 : 0;
+    return a.groups > 0 ? ((a.groups + a.units) * 16 * a.nq * (C + 1) + 2 * a.units + 1) * 4 : 0;
 }
 
 // How expanded_attention is launched.

@@ -341,6 +341,22 @@ def test_many_keys_and_many_rows(gpu, B, L, R, C, DR, P, W):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,L,R,C,DR,P,W,lens", [(200, 1, 20, 256, 32, 64, 16, "even"), (300, 1, 4, 512, 64, 16, 64, "ragged"), (260, 1, 16, 512, 32, 16, 40, "few"),
+                                                 (130, 2, 24, 256, 64, 32, 20, "ragged"), (7, 3, 50, 128, 32, 32, 50, "ragged"), (70, 1, 3, 512, 64, 16, 40, "none"),
+                                                 (2, 700, 3, 128, 64, 64, 30, "ragged"), (1, 9, 16, 512, 64, 16, 300, "even"), (90, 1, 40, 256, 32, 16, 60, "few")])
+def test_shares_of_many_sequences(gpu, B, L, R, C, DR, P, W, lens):
+    # both ways to share out keys, and a launch where there is nothing to share out
+    p = Problem(B, L, R, C, DR, P, W, F16, seed=B + R)
+    most = P * W - L
+    p.starts = [{"even": most, "ragged": (most * (b * 37 % 101)) // 100, "few": most if b % 29 == 3 else -L, "none": -L}[lens] for b in range(B)]
+    p.lens = [L if b % 3 else max(1, L // 2) for b in range(B)]
+    assert capi.latent_attention_plan(B, L, R, C, DR, P, W)["shared"] == 1
+    first = _compare(gpu, p)
+    again = _compare(gpu, p)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("C,DR,R,L,W", [(128, 32, 4, 1, 3), (512, 64, 16, 1, 60), (512, 64, 40, 2, 30), (256, 64, 16, 9, 4), (128, 64, 8, 40, 5)])
 def test_what_is_not_finite_stays_where_it_is_seen(gpu, dtype, C, DR, R, L, W):
