@@ -6,7 +6,10 @@ Two ways in, both ending in the same hand-written HIP kernels:
   the compiled torch binding, a drop-in for the reference's extension module (reference
   src/fused_attn_extention.cu:119-129).  ``attention_forward`` is re-exported here.
   The module also has ``attention_forward_ex`` and ``qkv_projection``, and for answering token by
-  token ``cache_append``, ``cached_attention`` and ``select_pages`` over a paged 8-bit cache.
+  token ``cache_append``, ``cached_attention`` and ``select_pages`` over a paged 8-bit cache,
+  ``latent_append``, ``latent_attention`` and ``expanded_attention`` for models that keep one latent
+  vector a token, ``rotary_tables`` and ``rotate`` for positions, and ``take_pages``, ``fork_pages``,
+  ``free_pages``, ``compact_pages`` and ``copy_pages`` for either cache's pages.
 * ``fused_attention_amd.capi`` -- a ctypes view of the C ABI declared in include/fused_attn.h,
   for callers that hold raw device pointers or a strided ``[B, R, L, H]`` tensor.
 

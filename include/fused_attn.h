@@ -463,7 +463,8 @@ int fa_latent_append(const fa_latent_cache* cache, const void* c, int64_t c_stri
  *     s_j = scale * (q . c_j + r . k_j),   out = sum_j softmax(s)_j c_j   (latent_dim; the head's map to values is the caller's)
  * over the cached tokens that fa_cached_attention would see: starts[b] + i + 1 with FA_FLAG_CAUSAL, otherwise starts[b] + new_lens[b], of
  * those on a page.  q, r and out [sequences, L, R, .] by strides of their own.  Rows that see nothing, and those of tokens that do not
- * exist, are zeros with an lse of -inf.  lse (nullable): float32 [sequences, R, L].  Scores, sums and outputs are float32; weights are rounded to the cache's type once.
+ * exist, are zeros with an lse of -inf.  lse (nullable): float32 [sequences, R, L].  Scores and sums are float32; weights,
+ * and the outputs, are rounded to the cache's type once.
  * fp16 weights keep 11 bits down to 2^-22 of the row's largest and lose what is below 2^-32.  A latent or rotary key that is not finite makes rows
  * that see it NaN where the formula does, or wholly; others never meet it.
  * workspace: fa_latent_attention_workspace bytes, 16-byte aligned, of no other call at the same time (nullable where that is 0).  The launch is
