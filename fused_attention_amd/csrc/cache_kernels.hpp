@@ -89,6 +89,19 @@ __device__ __forceinline__ float quad_sum(float x) {
     return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
 }
 
+// Of a wave's lanes: up to and with this one, and all.  Within rows of 16 lanes by 1, 2, 4 and 8, then the last lane of the first and third
+// row to the next, and of the second to the upper half; by way of LDS, six exchanges one after the other took 0.3 us.
+__device__ __forceinline__ int wave_sums(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_sums(x), 63); }
+
 // Between LDS accesses of the lanes of one wave to each other's places.  LDS serves a wave in order, so that nothing has to wait: this
 // keeps the compiler from exchanging them, and is no instruction.
 __device__ __forceinline__ void lanes_in_order() {

@@ -14,6 +14,7 @@ namespace pages {
 
 constexpr int kMostTensors = 8;
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kFew = 2048;               // pages whose list stays in LDS
 constexpr int kChunk = 256 * 4;          // units of a chunk of a page, four a thread
 
 struct Tensors {
@@ -67,12 +68,7 @@ struct Ranks {
 // this function's first.
 __device__ __forceinline__ Ranks rank_of(int n, int* room) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = n;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const int other = __shfl_up(sum, s);
-        if (lane >= s) sum += other;
-    }
+    const int sum = cache::wave_sums(n);
     __syncthreads();
     if (lane == 63) room[wave] = sum;
     __syncthreads();
@@ -168,56 +164,74 @@ struct TakeParams : View {
 };
 
 // One workgroup: the sequences' wants, the free pages in ascending order, and the pages to the places in the order of the rows.  Barriers
-// and loads one after the other, not bytes: 6.4 us for 18 sequences and 350 pages, 12.6 for 50 and 4500.
+// and loads one after the other, not bytes: 5.1 us for 18 sequences and 350 pages, 7.7 for 50 and 4500 (with the
+// sequences' places looked up row by row, and lists by way of memory, 6.4 and 12.6).
 __global__ __launch_bounds__(kPlanThreads) void take_pages_kernel(const TakeParams p) {
     __shared__ int room[kPlanWaves], wants[kPlanThreads];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    auto lacks = [&](int row, int64_t w, int64_t end) { return w < end && !p.is_page(p.table[row * p.table_stride + w]); };
+    __shared__ int from[kPlanThreads], upto[kPlanThreads], few[kFew];
+    // the places first .. last of row base + s that have no page: `got(w, before)` of each lane's, and how many
+    auto walk = [&](int base, int s, auto got) {
+        const int32_t* const entries = p.table + (base + s) * p.table_stride;
+        const int first = from[s], last = upto[s] < p.W ? upto[s] : p.W;
+        int n = 0;
+        for (int w0 = first; w0 < last; w0 += 4 * 64) {
+            int page[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int w = w0 + 64 * i + lane;
+                page[i] = w < last ? entries[w] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool lacks = !p.is_page(page[i]);
+                const uint64_t all = __ballot(lacks);
+                if (lacks) got(w0 + 64 * i + lane, n + __popcll(all & ((1ull << lane) - 1)));
+                n += __popcll(all);
+            }
+        }
+        return n;
+    };
     // twice over the rows, kPlanThreads at a time: what all want, then (found pages in `list`) who gets which
     int total = 0;
+    int* list = p.list;
     for (int pass = 0; pass < 2; ++pass) {
         int have = 0, given = 0;
         if (pass == 1) {
             if (total > p.N) total = p.N;
-            have = find_free(p, total, p.list, room);
+            if (total <= kFew) list = few;
+            have = find_free(p, total, list, room);
         }
         for (int base = 0; base < p.S; base += kPlanThreads) {
+            const int row = base + (int)threadIdx.x, rows = p.S - base < kPlanThreads ? p.S - base : kPlanThreads;
             __syncthreads();
-            for (int s = wave; s < kPlanThreads && base + s < p.S; s += kPlanWaves) {
+            if (row < p.S) {
                 int64_t first, end;
-                p.places(base + s, &first, &end);
-                const int64_t last = end < p.W ? end : p.W;
-                int n = 0;
-                for (int64_t w0 = first; w0 < last; w0 += 64) n += __popcll(__ballot(lacks(base + s, w0 + lane, last)));
+                p.places(row, &first, &end);
+                from[threadIdx.x] = (int)first, upto[threadIdx.x] = (int)end;
+            }
+            __syncthreads();
+            for (int s = wave; s < rows; s += kPlanWaves) {
+                const int n = walk(base, s, [](int, int) {});
                 if (lane == 0) wants[s] = n;
             }
             __syncthreads();
-            const Ranks r = rank_of(base + (int)threadIdx.x < p.S ? wants[threadIdx.x] : 0, room);
+            const Ranks r = rank_of(row < p.S ? wants[threadIdx.x] : 0, room);
             if (pass == 0) {
                 total = total + r.all < 0x40000000 ? total + r.all : 0x40000000;
                 continue;
             }
-            if (base + (int)threadIdx.x < p.S) wants[threadIdx.x] = given + r.before;      // the rank of its first
+            if (row < p.S) wants[threadIdx.x] = given + r.before;        // the rank of its first
             __syncthreads();
-            for (int s = wave; s < kPlanThreads && base + s < p.S; s += kPlanWaves) {
-                int64_t first, end;
-                p.places(base + s, &first, &end);
-                const int64_t last = end < p.W ? end : p.W;
-                int rank = wants[s];
-                int64_t without = end > (first > p.W ? first : (int64_t)p.W) ? end - (first > p.W ? first : (int64_t)p.W) : 0;
-                for (int64_t w0 = first; w0 < last; w0 += 64) {
-                    const bool mine = lacks(base + s, w0 + lane, last);
-                    const uint64_t all = __ballot(mine);
-                    const int at = rank + __popcll(all & ((1ull << lane) - 1));
-                    if (mine) {
-                        const int page = at < have ? p.list[at] : -1;
-                        p.table[(base + s) * p.table_stride + w0 + lane] = page;
-                        if (page >= 0) p.uses[page] = 1;
-                    }
-                    without += __popcll(__ballot(mine && at >= have));
-                    rank += __popcll(all);
-                }
-                if (lane == 0) p.missing[base + s] = (int)(without < 0x7fffffff ? without : 0x7fffffff);
+            for (int s = wave; s < rows; s += kPlanWaves) {
+                const int rank = wants[s], w = from[s] > p.W ? from[s] : p.W;
+                const int n = walk(base, s, [&](int w, int before) {
+                    const int page = rank + before < have ? list[rank + before] : -1;
+                    p.table[(base + s) * p.table_stride + w] = page;
+                    if (page >= 0) p.uses[page] = 1;
+                });
+                const int without = rank + n > have ? (rank > have ? n : rank + n - have) : 0;
+                if (lane == 0) p.missing[base + s] = without + (upto[s] > w ? upto[s] - w : 0);
             }
             given += r.all;
         }
@@ -243,7 +257,7 @@ __device__ __forceinline__ int unshared(const ForkParams& p, int parent, int len
     return p.is_page(page) ? page : -1;
 }
 
-// One workgroup: which pairs are forked, and the pages that they take.  Changes nothing but uses, of pages that were free.  5 to 7 us.
+// One workgroup: which pairs are forked, and the pages that they take.  Changes nothing but uses, of pages that were free.  4 to 6 us.
 __global__ __launch_bounds__(kPlanThreads) void plan_fork_kernel(const ForkParams p) {
     __shared__ int room[kPlanWaves];
     int total = 0;
@@ -319,34 +333,32 @@ struct CompactParams : View {
     Divisor by_width, by_chunks;
 };
 
-// One workgroup: the used pages are counted, U of them; the k-th hole among the first U pages takes the k-th used page behind them.  4.3 us for
-// 350 pages, 10.3 for 4500, barrier after barrier.
+// One workgroup: the used pages are counted, U of them; the k-th hole among the first U pages takes the k-th used page behind them.  3.3 us for
+// 350 pages, 7.9 for 4500, barrier after barrier.
 __global__ __launch_bounds__(kPlanThreads) void plan_compact_kernel(const CompactParams p) {
     __shared__ int room[kPlanWaves];
     constexpr int kEach = 4;
-    int U = 0;
+    int mine = 0;
     for (int base = 0; base < p.N; base += kEach * kPlanThreads) {
-        int n = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int page = base + i * kPlanThreads + (int)threadIdx.x;
-            n += page < p.N && p.uses[page] > 0;
+            mine += page < p.N && p.uses[page] > 0;
         }
-        U += rank_of(n, room).all;
     }
+    const int U = rank_of(mine, room).all;
     int holes = 0, movers = 0;
     for (int base = 0; base < p.N; base += kEach * kPlanThreads) {
         const int at = base + kEach * (int)threadIdx.x;
         bool used[kEach];
-        int h = 0, m = 0;
+        int n = 0;                                       // holes, and movers from bit 16 on: at most kEach * kPlanThreads of each
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             used[i] = at + i < p.N && p.uses[at + i] > 0;
-            h += at + i < U && !used[i];
-            m += at + i >= U && used[i];
+            n += at + i < U ? !used[i] : used[i] << 16;
         }
-        const Ranks rh = rank_of(h, room), rm = rank_of(m, room);
-        int hole = holes + rh.before, mover = movers + rm.before;
+        const Ranks r = rank_of(n, room);
+        int hole = holes + (r.before & 0xffff), mover = movers + (r.before >> 16);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if (at + i >= p.N) break;
@@ -354,8 +366,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_compact_kernel(const Compac
             if (at + i >= U && used[i]) p.movers[mover++] = at + i;
             if (at + i < U || !used[i]) p.moved[at + i] = used[i] ? at + i : -1;
         }
-        holes += rh.all;
-        movers += rm.all;
+        holes += r.all & 0xffff;
+        movers += r.all >> 16;
     }
     __syncthreads();                                     // both lists are written
     for (int k = threadIdx.x; k < holes; k += kPlanThreads) {
