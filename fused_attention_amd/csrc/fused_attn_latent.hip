@@ -113,19 +113,25 @@ int join_waves(int64_t parts) { return parts >= 32 ? 16 : parts >= 8 ? 4 : 1; }
 
 constexpr int64_t kMostParts = 128;          // of a row's keys
 
+// Rooms of LDS for tiles: two where that lets a third workgroup onto a compute unit that has one to take.
+int rooms_of(int nq, int64_t wgs, int64_t D) { return nq == 1 && D == 64 && wgs > 2 * kNumCu ? 2 : 3; }
+
 // Rows of a workgroup and parts of the keys by what a launch is estimated to take, causal (what the caller asks for is not known where the
 // workspace is sized): the longest workgroup's tiles, each `alone` us, or all tiles by what a compute unit takes for one, and the second
-// kernel's.  (Measured, with 128 and with 256 rows, us: 8 sequences of 1001 tokens of 12 heads of 64: 36, 38; 4 of them 27, 33; 2048
-// tokens of 16 heads of 128, 4 sequences 142, 111; one of 4096 118, 152; 4096 behind 12288, 32 heads 1357, 1067.)
+// kernel's.  (Measured, with 128 and with 256 rows, us: 8 sequences of 1001 tokens of 12 heads of 64: 32, 38; 4 of them 23, 33; 16 of 500 of
+// 16 heads 29, 27; 4 of 2048 of 16 heads 71, 78; 2048 tokens of 16 heads of 128, 4 sequences 142, 111; one of 4096 118, 152; 4096 behind 12288, 32 heads 1357, 1067.)
 Plan plan_expanded(int64_t B, int64_t L, int64_t R, int64_t K, int64_t D) {
     Plan best = {};
     float best_us = 3.0e38f;
-    const float longest = (float)ceil_div(K, kKeys), mean = K > L ? ((float)K - 0.5f * (float)L) / kKeys : 0.5f * longest;
+    const float longest = (float)ceil_div(K, kKeys), halfway = K > L ? ((float)K - 0.5f * (float)L) / kKeys : 0.5f * longest;
     for (int nq = 1; nq <= 2; ++nq) {
-        const float alone = D == 128 ? (nq == 2 ? 2.2f : 1.4f) : (nq == 2 ? 1.65f : 1.3f), each = D == 128 ? alone : (nq == 2 ? 1.65f : 0.9f);
+        const float alone = D == 128 ? (nq == 2 ? 2.2f : 1.4f) : (nq == 2 ? 1.65f : 1.3f);
         const int64_t tiles = ceil_div(L, kExpandedWaves * 16 * nq), base = B * R * tiles;
         for (int64_t s = 1; s <= kMostParts && (s == 1 || (base * s <= 4 * kNumCu && 2 * s <= ceil_div(K, kKeys))); s *= 2) {
-            const float chain = alone * (float)ceil_div((int64_t)longest, s), all = each * (float)base * (mean < longest ? mean : longest) / kNumCu;
+            const bool many = rooms_of(nq, base * s, D) == 2;
+            const float each = D == 128 ? alone : nq == 2 ? 1.9f : many ? 0.86f : 0.9f, begin = many ? 1.55f : 0.f;
+            const float mean = D == 128 ? halfway : halfway + (float)nq, steps = mean < longest ? mean : longest;
+            const float chain = alone * (float)ceil_div((int64_t)longest, s), all = (each * steps + begin * (float)s) * (float)base / kNumCu;
             const float join = s > 1 ? 4.f + (float)(B * L * R) * (float)(s * D) * 8.f / 2.5e6f : 0.f;
             const float us = 6.f + (chain > all ? chain : all) + join;
             if (us < best_us) best_us = us, best = {nq, tiles, s, base * s};
@@ -322,13 +328,22 @@ int fa_expanded_attention(const fa_expanded* x, float scale, int flags, void* wo
     p.by_heads = fa::divisor(R);
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto with = [&](auto d, auto dr, auto bf) {
-        auto run = [&](auto nq) {
-            auto kernel = expanded_attention_kernel<d(), dr(), bf(), nq()>;
-            constexpr int lds = Expanded<d(), dr()>::kLds;
+        auto run = [&](auto nq, auto rooms) {
+            auto kernel = expanded_attention_kernel<d(), dr(), bf(), nq(), rooms()>;
+            constexpr int lds = Expanded<d(), dr(), rooms()>::kLds;
             const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kernel), lds);
             return e != hipSuccess ? e : launch(kernel, a.wgs, 64 * kExpandedWaves, p, lds, s);
         };
-        const hipError_t e = a.nq == 1 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
+        auto in_rooms = [&]() {
+            constexpr std::integral_constant<int, 1> one;
+            constexpr std::integral_constant<int, 3> three;
+            if (a.nq == 2) return run(std::integral_constant<int, 2>{}, three);
+            if constexpr (d() == 64) {
+                if (rooms_of(a.nq, a.wgs, D) == 2) return run(one, std::integral_constant<int, 2>{});
+            }
+            return run(one, three);
+        };
+        const hipError_t e = in_rooms();
         if (e != hipSuccess || a.splits == 1) return e;
         const int waves = join_waves(a.splits);
         auto kernel = waves == 16 ? expanded_join_kernel<d(), bf(), 16> : waves == 4 ? expanded_join_kernel<d(), bf(), 4> : expanded_join_kernel<d(), bf(), 1>;

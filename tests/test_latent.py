@@ -505,6 +505,32 @@ def test_expanded_attention_of_long_prompts(gpu):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("DR", [32, 64])
+def test_expanded_attention_of_many_narrow_heads(gpu, dtype, DR):
+    # more than two workgroups of 128 rows for every compute unit; a sample of heads against the oracle
+    B, L, K, R, D = 3, 700, 731, 36, 64
+    starts, lens = [31, 0, -5], [700, 411, 700]
+    plan = capi.expanded_attention_plan(B, L, R, K, D, DR)
+    assert plan["rows"] == 128 and plan["workgroups"] > 512
+    for causal in (True, False):
+        got, lse, (q, k, kr, v, _, _, scale, _) = _expanded(gpu, B, L, K, R, D, DR, dtype, seed=DR, starts=starts, lens=lens, causal=causal)
+        for h in (0, 17, 35):
+            want = lo.expanded(q[:, :, h:h + 1], k[:, :, h:h + 1], kr, v[:, :, h:h + 1], starts, lens, scale, causal)
+            _check(got[:, :, h:h + 1], lse[:, h:h + 1], want, D + DR, K, dtype, v.abs().max().item())
+    # what only some rows see, and nobody
+    kv = torch.cat([k, v], -1)
+    bad, bad_r = kv.clone(), kr.clone()
+    bad[1, 411:], bad_r[1, 411:] = math.nan, math.inf
+    bad[0, 500, 4, D + 7] = math.inf
+    clean = _expanded(gpu, B, L, K, R, D, DR, dtype, seed=DR, starts=starts, lens=lens, kv=kv, kr=kr, q=q)[0].cpu()
+    got = _expanded(gpu, B, L, K, R, D, DR, dtype, seed=DR, starts=starts, lens=lens, kv=bad, kr=bad_r, q=q)[0].cpu()
+    hit = torch.zeros(B, L, R, D, dtype=torch.bool)
+    hit[0, 500 - 31:, 4, 7] = True
+    assert torch.equal(got[~hit], clean[~hit]) and not torch.isfinite(got[hit]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("L,K,D,DR", [(30, 100, 64, 32), (300, 300, 128, 64), (3, 2000, 128, 32)])
 def test_expanded_what_is_not_finite_stays_where_it_is_seen(gpu, dtype, L, K, D, DR):
     g = torch.Generator().manual_seed(7)
