@@ -109,7 +109,8 @@ int fa_take_pages(const fa_pages* c, const int32_t* new_lens, int64_t L, int32_t
     const int rc = check_keeping(c, true, &p);
     if (rc != FA_OK) return rc;
     if (L < 1) return FA_ERR_BAD_SHAPE;
-    if (L > kMaxInt) return FA_ERR_TOO_LARGE;
+    // the places of the whole table are counted in 32 bits: what every row wants, and the rank of each among all
+    if (L > kMaxInt || !below(c->sequences, c->table_width, kMaxInt)) return FA_ERR_TOO_LARGE;
     if (missing == nullptr) return FA_ERR_NULL_POINTER;
     if (!aligned(missing, 4) || !aligned(new_lens, 4)) return FA_ERR_MISALIGNED;
     if (workspace == nullptr || workspace_bytes < fa_take_pages_workspace(c)) return FA_ERR_WORKSPACE;

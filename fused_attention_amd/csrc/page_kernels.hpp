@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kPlanThreads) void take_pages_kernel(const TakePara
             __syncthreads();
             const Ranks r = rank_of(row < p.S ? wants[threadIdx.x] : 0, room);
             if (pass == 0) {
-                total = total + r.all < 0x40000000 ? total + r.all : 0x40000000;
+                total += r.all;                          // at most the table's places, as every sum here
                 continue;
             }
             if (row < p.S) wants[threadIdx.x] = given + r.before;        // the rank of its first

@@ -407,7 +407,8 @@ int fa_free_pages(const fa_pages* pages, const int32_t* sequences, int64_t count
  * Pages for new tokens: sequence b brings new_lens[b] of them (nullable: L; within [0, L]), behind starts[b].  The places
  * ceil(starts[b] / page_size) .. ceil((starts[b] + new_lens[b]) / page_size) of its row that name no page get the lowest free ones, in the
  * order of the rows and places, and a use each.  missing, int32 [sequences], receives how many places found no page or lie behind
- * the table; starts are left to the caller.  workspace: fa_take_pages_workspace bytes, 16-byte aligned, of no other call at the same time.
+ * the table; starts are left to the caller.  The table has fewer than 2^31 - 2^16 places, sequences * table_width (FA_ERR_TOO_LARGE).
+ * workspace: fa_take_pages_workspace bytes, 16-byte aligned, of no other call at the same time.
  */
 int fa_take_pages(const fa_pages* pages, const int32_t* new_lens, int64_t L, int32_t* missing, void* workspace, int64_t workspace_bytes,
                   void* stream);

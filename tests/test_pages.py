@@ -92,6 +92,15 @@ def test_the_library_refuses_what_its_header_says():
     assert lib.fa_take_pages_workspace(pages(pages=0)) == -3 and lib.fa_fork_pages_workspace(-1) == -3 and lib.fa_fork_pages_workspace(5000) == -6
 
 
+@pytest.mark.parametrize("S,W", [(140000, 16384), (1 << 20, 2048), (1 << 16, 32767)])
+def test_tables_whose_places_32_bits_cannot_count(S, W):
+    # refused from the sizes alone; 2^31 - 2^16 - 1 places are the most
+    ok = 0x1000
+    c = capi.Pages(page_table=ok, starts=ok, uses=ok, pages=10, page_size=16, sequences=S, table_width=W, table_stride=W)
+    assert S * W >= 2 ** 31 - 2 ** 16
+    assert capi.load_library().fa_take_pages(ctypes.byref(c), None, 1, ok, ok, 40, None) == -6
+
+
 @pytest.mark.parametrize("how", ["module", "capi"])
 def test_the_entry_points_refuse_wrong_tensors(how):
     m = _module() if how == "module" else capi
