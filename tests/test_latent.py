@@ -413,6 +413,77 @@ def test_scores_that_rise_and_fall(gpu, dtype, R, C, DR):
     _compare(gpu, p)
 
 
+def _end_to_end(p):
+    """Whether the workgroups lay the key tiles of all sequences end to end (causal calls): equal parts of a sequence's keys need more workgroups than
+    there are, or make one of them have too much.  A restatement of what each workgroup works out from the lengths."""
+    plan = capi.latent_attention_plan(p.B, p.L, p.R, p.C, p.DR, p.P, p.W)
+    tiles, steps = -(-p.L * p.R // plan["rows"]), -(-p.W * p.P // 64)
+    groups = min(p.B * tiles * -(-steps // 2), 512 if p.C == 128 else 256)
+    of = [-(-max(0, min(start + n, p.W * p.P)) // 64) if n > 0 else 0 for start, n in zip(p.starts, p.lens)]
+    share = max(2, -(-sum(of) * tiles // groups))
+    fits = [part for part in (share + (share * t + 7) // 8 for t in range(16)) if sum(-(-n // part) for n in of) * tiles <= groups]
+    return not fits or fits[0] > share + 5
+
+
+def _unseen(p):
+    """[pages, P]: the places of the cache that no row of a call sees."""
+    unseen = torch.ones(p.cache.shape[:2], dtype=torch.bool)
+    for b in range(p.B):
+        pos = torch.arange(max(0, min(p.starts[b] + p.lens[b], p.W * p.P)) if p.lens[b] > 0 else 0)
+        unseen[p.table[b, pos // p.P].long(), pos % p.P] = False
+    return unseen
+
+
+WIDE = [(16, 33, 16, 512, 64, 16, 40, "parts"), (2, 100, 16, 512, 32, 32, 64, "parts"), (60, 20, 16, 512, 64, 16, 20, "end to end"),
+        (60, 20, 16, 512, 32, 16, 20, "end to end"), (16, 128, 16, 512, 64, 16, 12, "alone"), (16, 128, 16, 512, 32, 16, 12, "alone"),
+        (10, 40, 16, 256, 32, 16, 40, "parts"), (60, 20, 16, 256, 64, 16, 24, "end to end"), (8, 128, 16, 256, 64, 16, 16, "alone"),
+        (20, 40, 16, 128, 32, 16, 40, "parts"), (110, 20, 16, 128, 32, 16, 36, "end to end"), (16, 128, 16, 128, 64, 16, 16, "alone")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,L,R,C,DR,P,W,way", WIDE)
+def test_workgroups_of_64_rows(gpu, dtype, B, L, R, C, DR, P, W, way):
+    # each way to share keys out and none, ragged lengths, scores that rise and fall from page to page
+    p = Problem(B, L, R, C, DR, P, W, dtype, seed=B + C)
+    most = P * W - L
+    p.starts = [most if b % 4 == 0 else (most * (b * 37 % 101)) // 100 for b in range(B)]
+    p.lens = [L if b % 3 else max(1, L // 2 + 1) for b in range(B)]
+    if B > 8:
+        p.starts[5], p.lens[6] = -L, 0                             # a sequence that sees nothing, and one without tokens
+    p.cache = (p.cache.float() * (0.05 + 2.0 * (torch.arange(p.cache.shape[0]) * 7 % 13) / 13)[:, None, None]).to(dtype)
+    plan = capi.latent_attention_plan(B, L, R, C, DR, P, W)
+    assert plan["rows"] == 64 and plan["shared"] == (way != "alone")
+    if way != "alone":
+        assert _end_to_end(p) == (way == "end to end")
+    clean = _compare(gpu, p)
+    _compare(gpu, p, causal=False)
+    again = _compare(gpu, p)
+    assert torch.equal(again[0], clean[0]) and torch.equal(again[1], clean[1])
+    # what nobody sees may be anything, and what some rows see reaches no others
+    unseen = _unseen(p)
+    bad = p.cache.clone()
+    bad[unseen] = torch.tensor([math.nan, math.inf, -math.inf], dtype=dtype)[torch.arange(int(unseen.sum())) % 3][:, None]
+    t = p.on(gpu)
+    for b, i, channel, value in ((0, L // 3, None, None), (0, L // 3, 5, math.nan), (1, L // 2, C - 1, math.inf), (0, L // 2, C + 1, math.nan)):
+        cache = bad.clone()
+        pos = p.starts[b] + i
+        if channel is not None:
+            cache[p.table[b, pos // P], pos % P, channel] = value
+        t["latent_cache"] = cache.to(gpu)
+        out, lse = _module().latent_attention(p.q.to(gpu), p.r.to(gpu), scale=p.scale, return_lse=True, **t)
+        sees = torch.zeros(B, L, dtype=torch.bool)
+        if channel is not None:
+            sees[b, i:p.lens[b]] = True
+            assert sees.any()
+        assert torch.equal(out.cpu()[~sees], clean[0].cpu()[~sees])
+        assert torch.equal(lse.cpu().transpose(1, 2)[~sees], clean[1].cpu().transpose(1, 2)[~sees])
+        if channel is not None and channel < C:
+            assert not torch.isfinite(out.cpu()[sees][..., channel]).any()
+        elif channel is not None:
+            assert torch.isnan(out.cpu()[sees]).all()
+
+
 @pytest.mark.gpu
 def test_views_and_tables_with_rows_apart(gpu):
     p = Problem(3, 2, 6, 256, 32, 32, 7, F16, seed=11)
@@ -559,6 +630,55 @@ def test_expanded_what_is_not_finite_stays_where_it_is_seen(gpu, dtype, L, K, D,
         hit = torch.zeros(2, L, 2, D, dtype=torch.bool)
         hit[b, at - starts[b]:, h] = True
         assert torch.equal(got.cpu()[~hit], clean.cpu()[~hit]) and torch.isnan(got.cpu()[hit]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,DR", [(64, 32), (64, 64), (128, 32), (128, 64)])
+def test_expanded_workgroups_of_256_rows(gpu, dtype, D, DR):
+    # two blocks of rows a wave: ragged lengths, row tiles without a token, causal or not; a sample of heads against the oracle
+    B, L, K, R = (5, 500, 520, 36) if D == 64 else (3, 520, 820, 40)
+    assert capi.expanded_attention_plan(B, L, R, K, D, DR)["rows"] == 256
+    starts, lens = [K - L, 0, 11, K - 1, -4][:B], [L, L - 30, 200, L, L][:B]
+    heads = (0, 21, R - 1)
+    for causal in (False, True):
+        got, lse, (q, k, kr, v, _, _, scale, _) = _expanded(gpu, B, L, K, R, D, DR, dtype, seed=D + DR, starts=starts, lens=lens, causal=causal)
+        for h in heads:
+            want = lo.expanded(q[:, :, h:h + 1], k[:, :, h:h + 1], kr, v[:, :, h:h + 1], starts, lens, scale, causal)
+            _check(got[:, :, h:h + 1], lse[:, h:h + 1], want, D + DR, K, dtype, v.abs().max().item())
+    got, lse = got.cpu(), lse.cpu()
+    # behind what anybody sees, and a value and a key that some rows see
+    bad, bad_r = torch.cat([k, v], -1), kr.clone()
+    for b in range(B):
+        bad[b, starts[b] + lens[b]:], bad_r[b, starts[b] + lens[b]:] = math.nan, -math.inf
+        bad[b, starts[b] + lens[b] + 1::2] = math.inf
+    for b, i, h, channel in ((None,) * 4, (0, 300, 21, D + 3), (1, L - 31, 0, 2 * D - 1), (2, 7, R - 1, 5)):
+        one, hit, all_of = bad.clone(), torch.zeros(B, L, R, D, dtype=torch.bool), torch.zeros(B, R, L, dtype=torch.bool)
+        if b is not None:
+            one[b, starts[b] + i, h, channel] = math.nan
+            hit[b, i:lens[b], h, channel - D if channel >= D else slice(None)] = True
+            all_of[b, h, i:lens[b]] = channel < D
+        out, sums, _ = _expanded(gpu, B, L, K, R, D, DR, dtype, seed=0, starts=starts, lens=lens, kv=one, kr=bad_r, q=q)
+        out, sums = out.cpu(), sums.cpu()
+        assert torch.equal(out[~hit], got[~hit]) and torch.isnan(out[hit]).all()
+        assert torch.equal(sums[~all_of], lse[~all_of]) and torch.isnan(sums[all_of]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("L,R,K,D,DR,splits", [(300, 2, 8192, 64, 32, 32), (1, 1, 16384, 64, 64, 128), (1, 1, 16384, 128, 64, 128), (1, 4, 16384, 128, 32, 64),
+                                                 (1000, 8, 16384, 128, 64, 8), (1000, 8, 16384, 128, 32, 8)])
+def test_expanded_keys_in_many_parts(gpu, dtype, L, R, K, D, DR, splits):
+    # joined by sixteen waves a row, or parts of 256 rows; parts that no row sees among them; the first and the last head against the oracle
+    plan = capi.expanded_attention_plan(1, L, R, K, D, DR)
+    assert plan["splits"] == splits and plan["rows"] == (256 if splits == 8 else 128)
+    for starts in ([K - L], [K // 3], [-1]):
+        got, lse, (q, k, kr, v, _, lens, scale, causal) = _expanded(gpu, 1, L, K, R, D, DR, dtype, seed=splits, starts=starts)
+        for h in {0, R - 1}:
+            want = lo.expanded(q[:, :, h:h + 1], k[:, :, h:h + 1], kr, v[:, :, h:h + 1], starts, lens, scale, causal)
+            _check(got[:, :, h:h + 1], lse[:, h:h + 1], want, D + DR, K, dtype, v.abs().max().item())
+        again = _expanded(gpu, 1, L, K, R, D, DR, dtype, seed=splits, starts=starts)
+        assert torch.equal(again[0], got) and torch.equal(again[1], lse)
 
 
 @pytest.mark.gpu

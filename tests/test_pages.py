@@ -235,6 +235,29 @@ def test_more_pages_and_sequences_than_threads(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N,enough", [(9001, True), (5000, False)])
+@pytest.mark.parametrize("how", ["module", "capi"])
+def test_more_pages_taken_at_once_than_stay_in_a_workgroup(gpu, N, enough, how):
+    # above 2048 wanted pages the free ones are listed in the workspace: with enough of them, and running out in the middle of a row
+    both = Both(gpu, 2500, 3, N, 16, seed=N, shapes=(((8,), torch.float16),))
+    m = _module() if how == "module" else capi
+    held = list(range(0, N, 7))[:300]                              # some pages are somebody's already
+    for n, page in enumerate(held):
+        both.k.table[8 * n][0], both.k.uses[page] = page, 1
+    both.table.copy_(_ints(both.k.table))
+    both.uses.copy_(_ints(both.k.uses))
+    lens = [17 + n * 7 % 24 for n in range(2500)]
+    wanted = sum(-(-n // 16) - (s % 8 == 0 and s // 8 < len(held)) for s, n in enumerate(lens))
+    assert wanted > 2048 and (wanted <= N - len(held)) == enough
+    got = m.take_pages(both.table, both.starts, both.uses, 16, 40, _ints(lens, gpu))
+    assert got.tolist() == both.k.take(lens, 40) and (int(got.sum()) == 0) == enough
+    both.check()
+    more = m.take_pages(both.table, both.starts, both.uses, 16, 48)      # places that stayed empty, and one more of many rows
+    assert more.tolist() == both.k.take([48] * 2500, 48)
+    both.check()
+
+
+@pytest.mark.gpu
 def test_lists_of_nothing_and_pages_beyond_32_bits(gpu):
     m = _module()
     both = Both(gpu, 3, 3, 6, 16, seed=2)

@@ -216,6 +216,29 @@ def test_rotation_of_many_rows(gpu, B, L, R, Rkv, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,layout,interleaved,inverse,first,dims", [(F16, "blf", False, True, 40, 64), (BF16, "bhld", True, False, 0, 128), (F16, "bhld", True, True, 96, 32),
+                                                                         (BF16, "blf", False, False, 24, 96)])
+def test_rotation_of_four_heads_a_thread(gpu, dtype, layout, interleaved, inverse, first, dims):
+    # enough heads of 16 channels that a thread takes four of them; head counts that are no multiple of it, copied channels, absent tokens, in place
+    B, L, R, Rkv, H = 2, 4100, 37, 6, 128
+    assert B * L * (R + Rkv) * (H // 16) >= 4 * 2048 * 256
+    q, k = _case(dtype, B, L, R, Rkv, H, layout, seed=dims)
+    cos, sin = (torch.from_numpy(x).float() for x in ro.tables(4096, dims))
+    starts, lens = torch.tensor([-3, 70], dtype=torch.int32), torch.tensor([4100, 3001], dtype=torch.int32)
+    exists = torch.arange(L)[None] < lens[:, None]
+    kw = dict(first=first, interleaved=interleaved, inverse=inverse)
+    want = [ro.rotate(_by_token(x, H, layout), cos, sin, starts[:, None] + torch.arange(L), exists=exists, **kw) for x in (q, k)]
+    dq, dk, dc, ds, dst, dl = (x.to(gpu) for x in (q, k, cos, sin, starts, lens))
+    m = _module()
+    calls = [m.rotate(dq, dc, ds, H, keys=dk, starts=dst, new_lens=dl, layout=layout, **kw),
+             capi.rotate(dq, (dc, ds), H, keys=dk, starts=dst, new_lens=dl, layout=layout, **kw),
+             m.rotate(dq, dc, ds, H, keys=dk, starts=dst, new_lens=dl, layout=layout, in_place=True, **kw)]
+    for got in calls:
+        for x, w in zip(got, want):
+            assert torch.equal(_by_token(x.cpu(), H, layout), w)
+
+
+@pytest.mark.gpu
 def test_rotation_is_the_caches(gpu):
     # the same tables give the same queries as appending to the 8-bit cache does
     m = _module()
