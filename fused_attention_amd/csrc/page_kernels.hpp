@@ -301,7 +301,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_fork_kernel(const ForkParam
 __global__ __launch_bounds__(256) void fork_pages_kernel(const ForkParams p) {
     const int per = 1 + p.tensors.first_chunk[p.tensors.count], n = (int)(blockIdx.x / per), part = (int)(blockIdx.x % per);
     const int length = p.lengths[n], copy = p.copies[n];
-    if (length <= 0) return;
+    if (length < 0) return;                              // not forked; of a parent without tokens the child's row is cleared all the same
     const int parent = p.parents[n], child = p.children[n];
     if (part > 0) {
         if (copy >= 0) copy_chunk(p.tensors, part - 1, unshared(p, parent, length), copy);

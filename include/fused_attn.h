@@ -419,7 +419,8 @@ int64_t fa_take_pages_workspace(const fa_pages* pages);
  * parent's last page is not full the child gets a copy of it in the lowest free page (those of smaller n first).  Its starts
  * become the parent's.  forked, int32 [count], receives 1; 0, and nothing else happens, where one of the two is no sequence, both are the same,
  * the child has tokens, smaller n name the child as well, or no page is free for the copy.  All parents are as before the call.  Pages that
- * an empty child's row names lose a use.  count is at most 4096 (FA_ERR_TOO_LARGE).  workspace as above.
+ * an empty child's row names lose a use, also where the parent has no tokens and the row becomes -1.  count is at most 4096
+ * (FA_ERR_TOO_LARGE).  workspace as above.
  */
 int fa_fork_pages(const fa_pages* pages, const int32_t* parents, const int32_t* children, int64_t count, int32_t* forked, void* workspace,
                   int64_t workspace_bytes, void* stream);

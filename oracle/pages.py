@@ -75,7 +75,7 @@ class Keeper:
                 else:
                     ok = False
             forked.append(int(ok))
-            if not ok or n == 0:
+            if not ok:
                 continue
             for page in self.table[child]:
                 if self.is_page(page):

@@ -41,6 +41,13 @@ def test_operations_of_the_oracle():
     assert k.holds[5] == 2 and k.holds[0] == 2
 
 
+def test_a_fork_of_a_sequence_without_tokens_in_the_oracle():
+    # the child goes on from nothing, and what its row named before is given back
+    k = Keeper([[-1, -1], [3, 1], [0, -1]], [0, 0, -5], [1, 1, 0, 1], 16)
+    assert k.fork([0, 2], [1, 0]) == [1, 1]
+    assert k.table == [[-1, -1], [-1, -1], [0, -1]] and k.uses == [1, 0, 0, 0] and k.starts == [0, 0, -5] and k.check()
+
+
 # ---- refusals, on the CPU ----
 
 def test_the_library_refuses_what_its_header_says():
@@ -254,6 +261,27 @@ def test_more_pages_taken_at_once_than_stay_in_a_workgroup(gpu, N, enough, how):
     both.check()
     more = m.take_pages(both.table, both.starts, both.uses, 16, 48)      # places that stayed empty, and one more of many rows
     assert more.tolist() == both.k.take([48] * 2500, 48)
+    both.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["module", "capi"])
+def test_a_fork_of_a_sequence_without_tokens(gpu, how):
+    # its child's row is cleared as any child's is, and pages that were taken for it, or that it shares, lose the use
+    m = _module() if how == "module" else capi
+    both = Both(gpu, 6, 4, 30, 16, seed=5)
+    k, args = both.k, (both.table, both.starts, both.uses)
+    lens = [0, 40, 17, 33, 0, 20]
+    assert m.take_pages(*args, 16, 40, _ints(lens, gpu)).tolist() == k.take(lens, 40)
+    both.starts[5] = k.starts[5] = 20                              # of those with pages only the last one gets tokens
+    both.starts[4] = k.starts[4] = -7
+    both.table[3, 3], k.table[3][3] = both.table[5, 0], k.table[5][0]
+    both.uses[k.table[5][0]] += 1
+    k.uses[k.table[5][0]] += 1
+    both.check()
+    parents, children = [0, 4, 5, 1], [1, 3, 2, 0]
+    assert m.fork_pages(both.tensors, *args, 16, _ints(parents, gpu), _ints(children, gpu)).tolist() == k.fork(parents, children) == [1, 1, 1, 1]
+    assert both.table[1].tolist() == [-1] * 4 and both.table[3].tolist() == [-1] * 4 and int((both.uses > 0).sum()) == 3 and int(both.uses.sum()) == 4
     both.check()
 
 
