@@ -34,6 +34,51 @@ bool turns_of(const fa_rotary* r, int64_t dims, double* turns) {
 
 bool is_positive(double x) { return x > 0 && std::isfinite(x); }
 
+// Rows of H values by their first address, strides and numbers.
+struct Rows {
+    const void* at;
+    Strides3 s;
+    int64_t B, heads, L;
+    bool same_places(const Rows& o) const {
+        return at == o.at && (B == 1 || s.b == o.s.b) && (heads == 1 || s.h == o.s.h) && (L == 1 || s.l == o.s.l);
+    }
+};
+struct Steps {
+    int64_t stride, least, most;
+};
+
+// Whether `d` is less than a row from a sum of so many of each stride.  A stride steps over all that those behind it reach, so that no more than two
+// numbers of steps come into question.
+bool reaches(int64_t d, const Steps* s, int n, int64_t H) {
+    if (n == 0) return -H < d && d < H;
+    const int64_t down = d / s->stride - (d % s->stride < 0 ? 1 : 0);
+    for (int64_t i : {down, down + 1}) {
+        i = std::min(std::max(i, s->least), s->most);
+        if (reaches(d - i * s->stride, s + 1, n - 1, H)) return true;
+    }
+    return false;
+}
+
+// Whether a row of `a` and one of `b` share a place.  Exact where both have the same strides, as views of one tensor have; otherwise it is looked whether the
+// first row of either is among the other's.
+bool meet(const Rows& a, const Rows& b, int64_t H) {
+    const int64_t strides[2][3] = {{a.s.b, a.s.h, a.s.l}, {b.s.b, b.s.h, b.s.l}}, counts[2][3] = {{a.B, a.heads, a.L}, {b.B, b.heads, b.L}};
+    const int64_t d = ((int64_t)reinterpret_cast<uintptr_t>(b.at) - (int64_t)reinterpret_cast<uintptr_t>(a.at)) / 2;
+    bool alike = true;
+    for (int i = 0; i < 3; ++i) alike = alike && (counts[0][i] == 1 || counts[1][i] == 1 || strides[0][i] == strides[1][i]);
+    auto within = [&](bool of_a, bool of_b) {
+        Steps steps[3];
+        int n = 0;
+        for (int i = 0; i < 3; ++i) {
+            const int64_t na = of_a ? counts[0][i] : 1, nb = of_b ? counts[1][i] : 1, stride = strides[na > 1 ? 0 : 1][i];
+            if ((na > 1 || nb > 1) && stride > 0) steps[n++] = {stride, 1 - nb, na - 1};
+        }
+        std::sort(steps, steps + n, [](const Steps& x, const Steps& y) { return x.stride > y.stride; });
+        return reaches(d, steps, n, H);
+    };
+    return alike ? within(true, true) : within(true, false) || within(false, true);
+}
+
 }  // namespace
 
 extern "C" {
@@ -97,6 +142,11 @@ int fa_rotate(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_s
         if (rc != FA_OK) return rc;
         t.chunks = (int)ceil_div(t.heads, heads);
     }
+    auto rows = [&](const void* t, const Strides3& strides, int64_t heads) { return Rows{t, strides, B, heads, L}; };
+    const Rows in[2] = {rows(q, p.of[0].xs, R), rows(k, p.of[1].xs, Rkv)}, written[2] = {rows(q_out, p.of[0].os, R), rows(k_out, p.of[1].os, Rkv)};
+    for (int n = 0; n < (k != nullptr ? 2 : 1); ++n)
+        if (!in[n].same_places(written[n]) && meet(in[n], written[n], H)) return FA_ERR_BAD_STRIDE;
+    if (k != nullptr && (meet(written[0], written[1], H) || meet(written[0], in[1], H) || meet(written[1], in[0], H))) return FA_ERR_BAD_STRIDE;
     p.B = (int)B;
     p.L = (int)L;
     p.H = (int)H;

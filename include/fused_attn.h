@@ -364,7 +364,8 @@ int fa_rotary_tables(float* cos, float* sin, int64_t rows, int64_t dims, const f
  * each product and each sum rounded to float32, the result to 16 bits.  cos / sin: float32 [rope_rows, dims / 2], 16-byte aligned.
  * Token i of sequence b has the position positions[b, i] (int32 [B, L], nullable) or starts[b] + i (int32 [B], nullable: zeros; not both:
  * FA_ERR_BAD_SHAPE).  Rows of tokens behind new_lens[b] (int32 [B], nullable), or whose position is outside [0, rope_rows), become
- * zeros.  out may be its input with the same strides; otherwise the two must not overlap, nor may q_out and k_out.
+ * zeros.  out may be its input with the same strides; otherwise the two must not overlap, nor may q_out and k_out, or one's output and the
+ * other's input (FA_ERR_BAD_STRIDE where both have the same strides, as views of one tensor, or the first row of either meets the other).
  */
 int fa_rotate(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, void* q_out, int64_t q_out_stride_b,
               int64_t q_out_stride_h, int64_t q_out_stride_l, const void* k, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_l,

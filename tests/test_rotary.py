@@ -7,6 +7,7 @@ product, the way back), the series by 7e-12, and the result is rounded once to f
 """
 import ctypes
 import math
+import random
 
 import numpy as np
 import pytest
@@ -101,6 +102,40 @@ def test_the_library_refuses_what_its_header_says():
     assert rotate(qs=(512, 64, 56)) == -4 and rotate(qs=(512, 60, 256)) == -4 and rotate(os=(512, 0, 256)) == -4 and rotate(os=(504, 64, 256)) == -4
     assert rotate(B=2 ** 20, L=2 ** 20) == -6 and rotate(L=2 ** 31) == -6
     assert rotate(k=ok, ks=(256, 64, 128), k_out=ok, kos=(256, 64, 64), Rkv=2) == -4 and rotate(k=ok, ks=(256, 64, 128), k_out=ok, kos=(256, 64, 128), Rkv=0) == -3
+
+
+def test_outputs_that_share_places_with_what_is_read_or_written_beside_them():
+    # against all places of small views, written out; without a GPU a call that is not refused ends at its launch
+    lib, ok, H = capi.load_library(), 0x100000, 16
+    g = random.Random(1)
+
+    def places(at, s, B, heads, L):
+        return {at // 2 + b * s[0] + h * s[1] + l * s[2] + c for b in range(B) for h in range(heads) for l in range(L) for c in range(H)}
+
+    seen = set()
+    for n in range(400):
+        B, L, R, Rkv = (g.choice([1, 2, 3]) for _ in range(4))
+        wide = g.choice([3, 4, 6]) * H                             # a token's values in the one tensor that all are views of
+        s = (wide * 5, H, wide)
+        at = [ok + 2 * (8 * g.randrange(0, 4 * H // 8) + wide * g.randrange(0, 3) + s[0] * g.randrange(0, 3)) for _ in range(4)]
+        if g.random() < 0.5:
+            at[1] = at[0]                                          # in place
+        if g.random() < 0.5:
+            at[3] = at[2]
+        if max(R, Rkv) * H > wide:
+            continue
+        of = [places(a, s, B, heads, L) for a, heads in zip(at, (R, R, Rkv, Rkv))]
+        bad = (at[0] != at[1] and of[0] & of[1]) or (at[2] != at[3] and of[2] & of[3]) or of[1] & of[3] or of[1] & of[2] or of[3] & of[0]
+        seen.add(bool(bad))
+        if bad or not torch.cuda.is_available():                   # (addresses of nothing: what is not refused goes to no GPU)
+            got = lib.fa_rotate(at[0], *s, at[1], *s, at[2], *s, at[3], *s, B, L, R, Rkv, H, 0, H, ok, ok, 9, None, None, None, 0, None)
+            assert got == -4 if bad else got > 0, (n, at, s, B, L, R, Rkv)
+    assert seen == {True, False}
+    one = lambda q_out, k, k_out, ks=(512, 64, 256): lib.fa_rotate(ok, 512, 64, 256, q_out, 512, 64, 256, k, *ks, k_out, *ks, 2, 2, 4, 1, 64, 0, 64, ok, ok, 9, None, None,
+                                                                   None, 0, None)
+    assert one(ok, ok, ok) == -4 and one(ok + 0x10000, ok, ok + 0x10000) == -4           # the same tensor twice, one output for both
+    assert one(ok, ok + 128, ok + 128, (64, 64, 64)) == -4                               # other strides, on one of the queries' heads
+    assert one(ok + 16, ok + 0x10000, ok + 0x10000) == -4                                # written 8 values behind what is read
 
 
 @pytest.mark.parametrize("how", ["module", "capi"])
@@ -283,6 +318,27 @@ def test_the_gradient_is_the_rotation_back(gpu, interleaved):
     leaf = y.clone().requires_grad_()
     f(leaf).backward()
     assert ((got.double() - leaf.grad).abs() <= leaf.grad.abs() * 2.0 ** -11 + 4 * 2.0 ** -24 * 8 + 2.0 ** -25).all()
+
+
+@pytest.mark.gpu
+def test_rotation_in_place_of_views_of_one_tensor(gpu):
+    m = _module()
+    B, L, H = 2, 5, 64
+    both = torch.randn(B, L, 8 * H, generator=torch.Generator().manual_seed(9)).to(BF16).to(gpu)
+    cos, sin = m.rotary_tables(16, H, gpu)
+    want_q, want_k = m.rotate(both[..., :4 * H], cos, sin, H, keys=both[..., 4 * H:6 * H])
+    kept = both.clone()
+    for call in (lambda q, k: m.rotate(q, cos, sin, H, keys=k, in_place=True), lambda q, k: capi.rotate(q, (cos, sin), H, keys=k, out=(q, k))):
+        for q, k in ((both, both), (both[..., :4 * H], both[..., 3 * H:5 * H]), (both[:, 1:], both[:, :-1])):
+            with pytest.raises(RuntimeError, match="stride"):
+                call(q, k)
+        assert torch.equal(both, kept)
+        call(both[..., :4 * H], both[..., 4 * H:6 * H])
+        assert torch.equal(both[..., :4 * H], want_q) and torch.equal(both[..., 4 * H:6 * H], want_k) and torch.equal(both[..., 6 * H:], kept[..., 6 * H:])
+        both.copy_(kept)
+    with pytest.raises(RuntimeError, match="stride"):              # each other's place
+        capi.rotate(both[..., :2 * H], (cos, sin), H, keys=both[..., 2 * H:4 * H], out=(both[..., 2 * H:4 * H], both[..., :2 * H]))
+    assert torch.equal(both, kept)
 
 
 @pytest.mark.gpu
