@@ -743,6 +743,8 @@ def rotate(queries, rope, head_dim, keys=None, starts=None, new_lens=None, posit
         if not isinstance(t, torch.Tensor) or t.shape != x.shape or t.dtype != x.dtype:
             raise ValueError("out must have the shape and dtype of what is rotated")
     outs_at = [_head_rows("out", t, layout, head_dim, queries)[3] for t in outs]
+    if out is not None and torch.is_grad_enabled() and any(t.requires_grad for t in outs):
+        raise ValueError("out requires a gradient, which the call does not record: rotate within a torch.autograd.Function, or under torch.no_grad()")
     _on_one_gpu(inputs + outs + [t for t in (cos, sin, starts, new_lens, positions) if t is not None])
     flags = _bf16(queries) | (FLAG_INTERLEAVED if interleaved else 0) | (FLAG_INVERSE if inverse else 0)
     k = (keys.data_ptr(), *shapes[1][3], outs[1].data_ptr(), *outs_at[1]) if keys is not None else (None, 0, 0, 0) * 2
@@ -751,6 +753,8 @@ def rotate(queries, rope, head_dim, keys=None, starts=None, new_lens=None, posit
             queries.data_ptr(), *shapes[0][3], outs[0].data_ptr(), *outs_at[0], *k, B, L, R, shapes[-1][2] if keys is not None else 0, head_dim,
             first, dims, cos.data_ptr(), sin.data_ptr(), rows, _address(positions), _address(starts), _address(new_lens), flags,
             _current_stream(queries) or None))
+    if out is not None:                                            # autograd sees that what it may have kept of them is gone
+        torch.autograd.graph.increment_version([t for t in outs if not t.is_inference()])
     return outs[0] if keys is None else tuple(outs)
 
 

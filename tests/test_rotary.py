@@ -104,6 +104,32 @@ def test_the_library_refuses_what_its_header_says():
     assert rotate(k=ok, ks=(256, 64, 128), k_out=ok, kos=(256, 64, 64), Rkv=2) == -4 and rotate(k=ok, ks=(256, 64, 128), k_out=ok, kos=(256, 64, 128), Rkv=0) == -3
 
 
+@pytest.mark.parametrize("how", ["module", "capi"])
+def test_in_place_refuses_what_autograd_would_go_on_with(how):
+    # its gradient would pass as if nothing had been rotated
+    errors = RuntimeError if how == "module" else ValueError
+    cos = torch.zeros(9, 16)
+
+    def call(q, k):
+        if how == "module":
+            return _module().rotate(q, cos, cos, 64, keys=k, in_place=True)
+        return capi.rotate(q, (cos, cos), 64, keys=k, out=(q, k))
+
+    def both():
+        return torch.zeros(2, 3, 256, dtype=F16), torch.zeros(2, 3, 128, dtype=F16)
+
+    for which in (0, 1):
+        x = both()
+        x[which].requires_grad_()
+        for y in (x, tuple(t * 1 for t in x)):                     # a leaf, and what follows from one
+            with pytest.raises(errors, match="gradient"):
+                call(*y)
+            with torch.no_grad(), pytest.raises(errors, match="GPU"):
+                call(*y)
+    with pytest.raises(errors, match="GPU"):
+        call(*both())
+
+
 def test_outputs_that_share_places_with_what_is_read_or_written_beside_them():
     # against all places of small views, written out; without a GPU a call that is not refused ends at its launch
     lib, ok, H = capi.load_library(), 0x100000, 16
@@ -339,6 +365,60 @@ def test_rotation_in_place_of_views_of_one_tensor(gpu):
     with pytest.raises(RuntimeError, match="stride"):              # each other's place
         capi.rotate(both[..., :2 * H], (cos, sin), H, keys=both[..., 2 * H:4 * H], out=(both[..., 2 * H:4 * H], both[..., :2 * H]))
     assert torch.equal(both, kept)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["module", "capi"])
+def test_autograd_sees_a_rotation_in_place(gpu, how):
+    cos, sin = capi.rotary_tables(8, 64, gpu)
+
+    def rotate(q, k, in_place):
+        if how == "module":
+            return _module().rotate(q, cos, sin, 64, keys=k, in_place=in_place)
+        return capi.rotate(q, (cos, sin), 64, keys=k, out=(q, k) if in_place else None)
+
+    w = torch.ones(1, 4, 192, dtype=F16, device=gpu, requires_grad=True)
+    both = torch.randn(1, 4, 192, generator=torch.Generator().manual_seed(2)).to(F16).to(gpu)
+    y = (w * both).float().sum()                                   # keeps `both` for the backward pass
+    versions = both._version
+    rotate(both[..., :128], both[..., 128:], False)
+    assert both._version == versions
+    rotate(both[..., :128], both[..., 128:], True)
+    assert both._version > versions
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        kept = both.clone()
+        rotate(kept[..., :128], kept[..., 128:], True)             # has no version
+    assert torch.equal(kept[..., :128], rotate(both[..., :128], both[..., 128:], False)[0])
+
+
+@pytest.mark.gpu
+def test_a_function_with_the_rotation_back_as_its_gradient(gpu):
+    # as a caller has it, in place of its input too: the gradient of both is that of the rotation written out
+    m = _module()
+    cos, sin = m.rotary_tables(8, 64, gpu)
+
+    class Rotate(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, in_place):
+            if in_place:
+                ctx.mark_dirty(x)
+            return m.rotate(x, cos, sin, 64, in_place=in_place)
+
+        @staticmethod
+        def backward(ctx, g):
+            return m.rotate(g.contiguous(), cos, sin, 64, inverse=True), None
+
+    g = torch.Generator().manual_seed(3)
+    x, w = (torch.randn(2, 5, 128, generator=g).to(BF16).to(gpu) for _ in range(2))
+    want = m.rotate(w, cos, sin, 64, inverse=True)
+    for in_place in (False, True):
+        leaf = x.clone().requires_grad_()
+        out = Rotate.apply(leaf * 1, in_place)
+        assert torch.equal(out, m.rotate(x, cos, sin, 64))
+        out.backward(w)
+        assert torch.equal(leaf.grad, want)
 
 
 @pytest.mark.gpu
