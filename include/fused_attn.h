@@ -382,6 +382,9 @@ int fa_rotate(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_s
  *   uses        int32 [pages]: how many entries of the table name the page; a page without uses is free
  *   data        `tensors` (up to 8) tensors of `pages` pages of page_bytes each, one behind the other: what a page holds
  *               (looked at by fa_copy_pages, fa_fork_pages and fa_compact_pages)
+ * Where one table keeps more tensors than a call takes, those of a model's other layers, fa_fork_pages and fa_compact_pages are called once all the
+ * same, for each of them changes the table and the uses: the other tensors' pages are then copied by fa_copy_pages, from every page to where `moved`
+ * says, and from the page that a forked parent's tokens end in, where they do not fill it, to the one at the same place of its child's row.
  *
  * Lists are int32 in device memory; numbers in them that are no sequence, or no page, are passed over.  A count of 0 does nothing.
  * Of a page's bytes 16 are moved at a time where the tensor is aligned to 16 and page_bytes is a multiple of it; otherwise 4, or 1.

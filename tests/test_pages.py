@@ -307,6 +307,46 @@ def test_lists_of_nothing_and_pages_beyond_32_bits(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how", ["module", "capi"])
+def test_pages_of_more_tensors_than_a_call_takes(gpu, how):
+    # the layers of a model: the first eight tensors go with the table, the others follow by copies
+    m = _module() if how == "module" else capi
+    P, S, W = 16, 14, 5
+    both = Both(gpu, S, W, 60, P, seed=6, shapes=(((16, 24), torch.float16), (7, torch.int8)) * 10)
+    k, args, rng = both.k, (both.table, both.starts, both.uses), random.Random(3)
+    everything = torch.arange(both.N, dtype=I32, device=gpu)
+    groups = [both.tensors[n:n + 8] for n in range(8, len(both.tensors), 8)]
+    assert [len(g) for g in groups] == [8, 4]
+    copied = 0
+    for turn in range(12):
+        gone = [rng.randrange(S) for _ in range(4)]
+        m.free_pages(*args, _ints(gone, gpu))
+        k.free(gone)
+        moved = m.compact_pages(both.tensors[:8], both.table, both.uses)
+        assert moved.tolist() == k.compact()
+        for rest in groups:
+            m.copy_pages(rest, everything, moved)
+        both.check()
+        lens = [rng.choice([0, 16, 23, 48]) if n % 2 else 0 for n in range(S)]
+        m.take_pages(*args, P, 48, _ints(lens, gpu))
+        k.take(lens, 48)
+        both.starts += _ints(lens, gpu)
+        k.starts = [a + b for a, b in zip(k.starts, lens)]
+        parents, children = [_ints([rng.randrange(S) for _ in range(9)], gpu) for _ in range(2)]
+        ok = m.fork_pages(both.tensors[:8], *args, P, parents, children)
+        assert ok.tolist() == k.fork(parents.tolist(), children.tolist())
+        tokens = both.starts[parents]
+        place = (tokens // P).clamp(max=both.table.shape[1] - 1)
+        last, copy = both.table[parents, place], both.table[children, place]
+        copy = torch.where((ok == 1) & (tokens % P != 0), copy, -1)
+        copied += int(((copy >= 0) & (last >= 0)).sum())
+        for rest in groups:
+            m.copy_pages(rest, last, copy)
+        both.check()
+    assert copied > 5
+
+
+@pytest.mark.gpu
 def test_a_turn_captured_in_a_graph(gpu):
     # a turn of a server, replayed: the lists' and the table's contents decide, as the host's steps do
     m = _module()
