@@ -42,6 +42,8 @@ struct Rows {
     bool same_places(const Rows& o) const {
         return at == o.at && (B == 1 || s.b == o.s.b) && (heads == 1 || s.h == o.s.h) && (L == 1 || s.l == o.s.l);
     }
+    uintptr_t begin() const { return reinterpret_cast<uintptr_t>(at); }
+    uintptr_t end(int64_t H) const { return begin() + 2 * (uintptr_t)((B - 1) * s.b + (heads - 1) * s.h + (L - 1) * s.l + H); }
 };
 struct Steps {
     int64_t stride, least, most;
@@ -62,6 +64,7 @@ bool reaches(int64_t d, const Steps* s, int n, int64_t H) {
 // Whether a row of `a` and one of `b` share a place.  Exact where both have the same strides, as views of one tensor have; otherwise it is looked whether the
 // first row of either is among the other's.
 bool meet(const Rows& a, const Rows& b, int64_t H) {
+    if (a.end(H) <= b.begin() || b.end(H) <= a.begin()) return false;        // new outputs
     const int64_t strides[2][3] = {{a.s.b, a.s.h, a.s.l}, {b.s.b, b.s.h, b.s.l}}, counts[2][3] = {{a.B, a.heads, a.L}, {b.B, b.heads, b.L}};
     const int64_t d = ((int64_t)reinterpret_cast<uintptr_t>(b.at) - (int64_t)reinterpret_cast<uintptr_t>(a.at)) / 2;
     bool alike = true;
