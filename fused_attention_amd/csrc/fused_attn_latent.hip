@@ -75,7 +75,8 @@ struct LatentPlan {
 
 // Rows of a workgroup by what a launch is estimated to take: tiles of 64 rows take less for each row, of 32 less to begin and to join.
 // (C = 512, us, 32 and 64 rows, with the joining: 16 sequences of 2000 tokens, 160 rows each 36, 38; 2 of them 22, 25; one of 32000
-// 35, 38; 128 rows of one of 131072 73, 65.)
+// 35, 38; 128 rows of one of 131072 73, 65.)  Both are for the table's width, the lengths being in device memory, and used for 128 and 256 channels too,
+// whose tiles take less than the estimate says.
 LatentPlan plan_latent(const View& p, int64_t C) {
     LatentPlan a;
     const int64_t rows = (int64_t)p.L * p.R, steps = ceil_div((int64_t)p.W << p.log2_p, kKeys), resident = (C == 128 ? 2 : 1) * kNumCu;
@@ -87,7 +88,9 @@ LatentPlan plan_latent(const View& p, int64_t C) {
     a.nq = rows <= 16 ? 1 : rows <= 32 || estimate(2) < estimate(4) ? 2 : 4;
     a.tiles = ceil_div(rows, 16 * a.nq);
     a.units = p.B * a.tiles;
-    // None shared out where one workgroup is through with its unit before a second kernel would be (C = 128, 4 tiles: 5 us, shared out 10).
+    // None shared out where one workgroup is through with its unit before a second kernel would be (C = 128, 4 tiles: 5 us, shared out 10), nor from two
+    // units for each place on: they even each other out where lengths are alike, but one long sequence is as slow as its own tiles are one after the
+    // other (512 of 1000 tokens, 16 rows, one of them of 131072: 3960 us; 511 of them, shared out, 158).
     a.groups = 0;
     if (a.units <= kMostUnits && a.units < 2 * resident && steps > 2 + 768 / C && below(steps, a.units, 0x3fffffff)) {
         const int64_t shares = a.units * ceil_div(steps, a.least_share);         // more have nothing to do

@@ -29,8 +29,8 @@ struct TablesParams {
 // Four columns of a row to a thread.  Angles are kept in turns: the whole ones fall away without an error, the quarters decide which of
 // the two series is the cosine and with what sign, and both run over at most an eighth of a turn, y in [-pi / 4, pi / 4], where
 // Taylor's series to y^11 and y^12 are within 7e-12.  All of it in 64 bits, one rounding at the end: at position 131071 the product of
-// position and frequency in float32 would be off by a thousandth of a turn.  131072 rows of 2 x 64: 17 us, 67 MB at 3.9 TB/s, which is a fill's
-// rate at that size; 8192 rows of 2 x 32 4 us, a launch.
+// position and frequency in float32 would be off by a thousandth of a turn.  131072 rows of 2 x 64: 17 us, 67 MB at 3.9 TB/s, where a fill
+// of that size reaches 6.0; 8192 rows of 2 x 32 4 us, a launch.
 __global__ __launch_bounds__(256) void rotary_tables_kernel(const TablesParams p) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int groups = p.half / 4;
